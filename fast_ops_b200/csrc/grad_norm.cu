@@ -1,0 +1,249 @@
+// The 2-norm over all elements of a list of gradients, and the factor that clips them to a norm:
+//
+//   norm = sqrt(sum_t sum_i g_t[i]^2)      coef = min(1, max_norm / (norm + 1e-6))
+//
+// Bound by HBM: every gradient is read once.  The tensor list travels in the kernel's arguments (no device
+// table, nothing cached, nothing allocated), so a call can be captured into a graph the first time it is made.
+//
+// A thread squares and sums eight elements in fp32 (the squares of 16-bit values are exact there) and adds
+// each such sum to a double, so that what the norm loses to rounding does not grow with the list.  Where
+// the fp32 sum of eight leaves the range in which its squares are normal numbers (gradients beyond 1e18 or
+// all below 1e-15), the eight are summed again in double.  Every sum is formed in a fixed order: the same
+// list gives the same bits on every run.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+#include <cstring>
+
+#include "fo_host.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kVec = 8;     // elements of one group: 16 bytes of a 16-bit type, 32 of fp32
+constexpr int kUnroll = 4;  // groups of a thread in flight
+constexpr int kChunk = kThreads * kVec * kUnroll;  // 8192 elements: what a block takes at a time
+
+// Most tensors of one launch: what fits the 32764 bytes of kernel arguments.  A longer list takes several
+// launches.  Short lists use the small form, whose arguments are a tenth as long.
+constexpr int kMaxTensors = 1024, kFewTensors = 96;
+
+template <int kMax>
+struct TensorList {
+  const void* ptr[kMax];
+  int64_t numel[kMax];
+  uint32_t first_chunk[kMax + 1];  // index of the tensor's first chunk among all chunks of the launch
+  uint8_t dtype[kMax];
+  int n;
+};
+
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+
+// Eight elements from a 16-byte aligned address.
+__device__ __forceinline__ void load8(const float* p, float (&v)[kVec]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[kVec]) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load8(const __half* p, float (&v)[kVec]) {
+  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __half2 h;
+    memcpy(&h, &w[i], 4);
+    const float2 f = __half22float2(h);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+__device__ __forceinline__ double sum_of_squares8(const float (&v)[kVec]) {
+  const float s = ((v[0] * v[0] + v[1] * v[1]) + (v[2] * v[2] + v[3] * v[3])) +
+                  ((v[4] * v[4] + v[5] * v[5]) + (v[6] * v[6] + v[7] * v[7]));
+  if (s > 1e-30f && s < 1e37f) return static_cast<double>(s);
+  double d = 0;  // zeros, tiny or huge values, infinities and NaN
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) d += static_cast<double>(v[i]) * static_cast<double>(v[i]);
+  return d;
+}
+
+// This thread's share of one chunk's sum: `left` elements of the tensor remain from `p` on.
+template <typename T>
+__device__ __forceinline__ double chunk_sum(const T* p, int64_t left) {
+  double sum = 0;
+  if (left >= kChunk && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    float v[kUnroll][kVec];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) load8(p + (u * kThreads + threadIdx.x) * kVec, v[u]);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) sum += sum_of_squares8(v[u]);
+  } else {
+    // the tail of a tensor, or one whose storage is not 16-byte aligned
+    const int n = left < kChunk ? static_cast<int>(left) : kChunk;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const double x = static_cast<double>(load1(p + i));
+      sum += x * x;
+    }
+  }
+  return sum;
+}
+
+// Sum over the block's threads, valid in thread 0; `scratch` holds one value per warp.
+__device__ __forceinline__ double block_sum(double v, double* scratch) {
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    v = threadIdx.x < kThreads / 32 ? scratch[threadIdx.x] : 0;
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  }
+  return v;
+}
+
+// partials[block] = the block's share of the sum of squares.
+template <int kMax>
+__global__ void __launch_bounds__(kThreads)
+grad_sumsq_kernel(const __grid_constant__ TensorList<kMax> list, double* __restrict__ partials) {
+  __shared__ double scratch[kThreads / 32];
+  const uint32_t total = list.first_chunk[list.n];
+  int t = 0;
+  double sum = 0;
+  for (uint32_t chunk = blockIdx.x; chunk < total; chunk += gridDim.x) {
+    while (chunk >= list.first_chunk[t + 1]) ++t;  // a block's chunks only go up
+    const int64_t base = static_cast<int64_t>(chunk - list.first_chunk[t]) * kChunk;
+    const int64_t left = list.numel[t] - base;
+    const int dtype = list.dtype[t];
+    if (dtype == FO_F32) sum += chunk_sum(static_cast<const float*>(list.ptr[t]) + base, left);
+    else if (dtype == FO_BF16) sum += chunk_sum(static_cast<const __nv_bfloat16*>(list.ptr[t]) + base, left);
+    else sum += chunk_sum(static_cast<const __half*>(list.ptr[t]) + base, left);
+  }
+  sum = block_sum(sum, scratch);
+  if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+}
+
+// One block: the sum of all partials, and norm and clipping factor from it.
+__global__ void __launch_bounds__(kThreads)
+grad_norm_finish_kernel(const double* __restrict__ partials, int n, float max_norm, double* __restrict__ sumsq,
+                        float* __restrict__ norm_coef) {
+  __shared__ double scratch[kThreads / 32];
+  double sum = 0;
+  for (int i = threadIdx.x; i < n; i += kThreads) sum += partials[i];
+  sum = block_sum(sum, scratch);
+  if (threadIdx.x != 0) return;
+  if (sumsq != nullptr) *sumsq = sum;
+  if (norm_coef != nullptr) {
+    const float norm = static_cast<float>(sqrt(sum));
+    const float coef = __fdiv_rn(max_norm, __fadd_rn(norm, 1e-6f));
+    norm_coef[0] = norm;
+    norm_coef[1] = coef > 1.f ? 1.f : coef;  // a NaN stays one
+  }
+}
+
+// Blocks of the widest launch: enough to fill the chip, and what the caller's workspace holds a double for.
+constexpr int kMaxBlocks = 148 * 8;
+
+template <int kMax>
+int launch_sumsq(const void* const* grads, const int64_t* numels, const int* dtypes, int begin, int end, double* partials,
+                 int room, int* blocks_out, cudaStream_t stream) {
+  TensorList<kMax> list;
+  int n = 0;
+  uint32_t chunks = 0;
+  for (int i = begin; i < end; ++i) {
+    if (numels[i] == 0) continue;
+    list.ptr[n] = grads[i];
+    list.numel[n] = numels[i];
+    list.dtype[n] = static_cast<uint8_t>(dtypes[i]);
+    list.first_chunk[n] = chunks;
+    chunks += static_cast<uint32_t>((numels[i] + kChunk - 1) / kChunk);
+    ++n;
+  }
+  *blocks_out = 0;
+  if (n == 0) return FO_OK;
+  list.first_chunk[n] = chunks;
+  list.n = n;
+  const int blocks = static_cast<int>(chunks < static_cast<uint32_t>(room) ? chunks : room);
+  grad_sumsq_kernel<kMax><<<blocks, kThreads, 0, stream>>>(list, partials);
+  fo::g_launch_count.fetch_add(1, std::memory_order_relaxed);
+  FO_CUDA_CHECK(cudaGetLastError());
+  *blocks_out = blocks;
+  return FO_OK;
+}
+
+int launch_finish(const double* partials, int n, float max_norm, double* sumsq, float* norm_coef, cudaStream_t stream) {
+  grad_norm_finish_kernel<<<1, kThreads, 0, stream>>>(partials, n, max_norm, sumsq, norm_coef);
+  fo::g_launch_count.fetch_add(1, std::memory_order_relaxed);
+  FO_CUDA_CHECK(cudaGetLastError());
+  return FO_OK;
+}
+
+int check_max_norm(double max_norm) {
+  FO_REQUIRE(max_norm >= 0.0, "max_norm must be non-negative (got %g)", max_norm);
+  return FO_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t fo_grad_norm_workspace(int n_tensors) {
+  const int64_t launches = n_tensors <= kMaxTensors ? 1 : (static_cast<int64_t>(n_tensors) + kMaxTensors - 1) / kMaxTensors;
+  return launches * kMaxBlocks;
+}
+
+extern "C" int fo_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int n_tensors,
+                            double max_norm, double* workspace, double* sumsq, float* norm_coef, int device, void* stream) {
+  fo::clear_error();
+  FO_REQUIRE(n_tensors >= 0, "n_tensors must be >= 0");
+  FO_REQUIRE(n_tensors == 0 || (grads && numels && dtypes), "null tensor list");
+  FO_REQUIRE(workspace != nullptr, "null workspace");
+  FO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 7) == 0, "workspace must be 8-byte aligned");
+  FO_REQUIRE(sumsq != nullptr || norm_coef != nullptr, "nowhere to put the result");
+  if (int rc = check_max_norm(max_norm)) return rc;
+  int64_t total = 0;
+  for (int i = 0; i < n_tensors; ++i) {
+    FO_REQUIRE(numels[i] >= 0, "tensor %d has negative numel", i);
+    FO_REQUIRE(numels[i] == 0 || grads[i] != nullptr, "tensor %d has a null pointer", i);
+    FO_REQUIRE(dtypes[i] == FO_F16 || dtypes[i] == FO_BF16 || dtypes[i] == FO_F32, "tensor %d: bad dtype %d", i, dtypes[i]);
+    FO_REQUIRE(numels[i] == 0 || reinterpret_cast<uintptr_t>(grads[i]) % (dtypes[i] == FO_F32 ? 4 : 2) == 0,
+               "tensor %d is not aligned to its elements", i);
+    FO_REQUIRE(numels[i] <= (int64_t{1} << 44), "tensor %d is too large", i);
+    total += (numels[i] + kChunk - 1) / kChunk;
+  }
+  FO_REQUIRE(total < (int64_t{1} << 31), "the list has too many elements");
+  fo::DeviceGuard guard(device);
+  FO_REQUIRE(guard.ok, "cannot make device %d current", device);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int used = 0;  // partials written so far
+  for (int begin = 0; begin < n_tensors; begin += kMaxTensors) {
+    const int end = n_tensors - begin < kMaxTensors ? n_tensors : begin + kMaxTensors;
+    int blocks = 0;
+    const int rc = end - begin <= kFewTensors
+                       ? launch_sumsq<kFewTensors>(grads, numels, dtypes, begin, end, workspace + used, kMaxBlocks, &blocks, s)
+                       : launch_sumsq<kMaxTensors>(grads, numels, dtypes, begin, end, workspace + used, kMaxBlocks, &blocks, s);
+    if (rc) return rc;
+    used += blocks;
+  }
+  return launch_finish(workspace, used, static_cast<float>(max_norm), sumsq, norm_coef, s);
+}
+
+extern "C" int fo_grad_norm_finish(const double* sumsq, double max_norm, float* norm_coef, int device, void* stream) {
+  fo::clear_error();
+  FO_REQUIRE(sumsq != nullptr && norm_coef != nullptr, "null pointer");
+  if (int rc = check_max_norm(max_norm)) return rc;
+  fo::DeviceGuard guard(device);
+  FO_REQUIRE(guard.ok, "cannot make device %d current", device);
+  return launch_finish(sumsq, 1, static_cast<float>(max_norm), nullptr, norm_coef, static_cast<cudaStream_t>(stream));
+}

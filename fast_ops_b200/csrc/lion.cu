@@ -54,6 +54,7 @@ struct LionConsts {
   float c_nlr;   // -lr, rounded to promote(p, m)
   float c_b2;    // beta2
   float c_1mb2;  // 1 - beta2, rounded to promote(p, m)
+  float clip;    // factor of the gradients; set inside the kernels that clip, from device memory
 };
 
 // ---- storage-type helpers -------------------------------------------------------------
@@ -104,12 +105,14 @@ __device__ __forceinline__ void store_group(T* dst, const Group<T>& src) {
   for (int i = 0; i < n16; ++i) __stcs(d + i, s[i]);
 }
 
-template <typename TP, typename TM>
+// kClip: the gradient is g * clip, rounded to its type once, as if it had been clipped in memory first.
+template <typename TP, typename TM, bool kClip = false>
 __device__ __forceinline__ void lion_element(TP& p_io, TP g_in, TM& m_io, const LionConsts& c) {
   using TG = TP;
   using TU = typename Promote<TM, TG>::type;
   const float p = Elem<TP>::load(p_io);
-  const float g = Elem<TG>::load(g_in);
+  float g = Elem<TG>::load(g_in);
+  if constexpr (kClip) g = Elem<TG>::round(__fmul_rn(g, c.clip));
   const float m = Elem<TM>::load(m_io);
   const float p1 = Elem<TP>::round(__fmul_rn(p, c.c_wd));
   const float t1 = Elem<TM>::round(__fmul_rn(m, c.c_b1));
@@ -126,16 +129,16 @@ __device__ __forceinline__ void lion_element(TP& p_io, TP g_in, TM& m_io, const 
 // compiler contracted the packed multiply and add into one fused multiply-add, which flips the
 // sign of beta1*m + (1-beta1)*g where the two rounded terms cancel exactly.  The scalar _rn
 // intrinsics below are never contracted.)
-template <typename TP, typename TM>
+template <typename TP, typename TM, bool kClip = false>
 __device__ __forceinline__ void lion_group(Group<TP>& pv, const Group<TP>& gv, Group<TM>& mv, const LionConsts& c) {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) lion_element<TP, TM>(pv.v[i], gv.v[i], mv.v[i], c);
+  for (int i = 0; i < kVec; ++i) lion_element<TP, TM, kClip>(pv.v[i], gv.v[i], mv.v[i], c);
 }
 
 // One chunk of kU * kThreads * kVec elements: `remaining` elements are left from p, g, m on (a full
 // chunk of them are this chunk's unless the tensor ends earlier); `aligned` says that all three
 // addresses allow 16-byte accesses.
-template <typename TP, typename TM, int kU = kUnroll>
+template <typename TP, typename TM, int kU = kUnroll, bool kClip = false>
 __device__ __forceinline__ void lion_chunk(TP* p, const TP* g, TM* m, int64_t remaining, bool aligned,
                                            const LionConsts& c) {
   constexpr int kElems = kThreads * kVec * kU;
@@ -151,7 +154,7 @@ __device__ __forceinline__ void lion_chunk(TP* p, const TP* g, TM* m, int64_t re
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
-      lion_group<TP, TM>(pv[u], gv[u], mv[u], c);
+      lion_group<TP, TM, kClip>(pv[u], gv[u], mv[u], c);
       const int off = (u * kThreads + threadIdx.x) * kVec;
       store_group(p + off, pv[u]);
       store_group(m + off, mv[u]);
@@ -162,7 +165,7 @@ __device__ __forceinline__ void lion_chunk(TP* p, const TP* g, TM* m, int64_t re
     for (int i = threadIdx.x; i < n; i += kThreads) {
       TP pe = p[i];
       TM me = m[i];
-      lion_element<TP, TM>(pe, g[i], me, c);
+      lion_element<TP, TM, kClip>(pe, g[i], me, c);
       p[i] = pe;
       m[i] = me;
     }
@@ -217,16 +220,17 @@ lion_table_walk_kernel(const LionTensor* __restrict__ tensors,
 // GPT-2-medium list with one wave, 6.56 with four, 6.05 with sixteen).
 constexpr int kSingleUnroll = 1;
 
-template <typename TP, typename TM>
+template <typename TP, typename TM, bool kClip>
 __global__ void __launch_bounds__(kThreads)
 lion_single_tensor_kernel(TP* __restrict__ p, const TP* __restrict__ g, TM* __restrict__ m, int64_t numel,
-                          int64_t total_chunks, LionConsts c) {
+                          int64_t total_chunks, LionConsts c, const float* __restrict__ clip) {
+  if constexpr (kClip) c.clip = __ldg(clip);
   constexpr int kU = kSingleUnroll;
   constexpr int kElems = kThreads * kVec * kU;
   const bool aligned = all_aligned16(p, g, m);
   for (int64_t chunk = blockIdx.x; chunk < total_chunks; chunk += gridDim.x) {
     const int64_t base = chunk * kElems;
-    lion_chunk<TP, TM, kU>(p + base, g + base, m + base, numel - base, aligned, c);
+    lion_chunk<TP, TM, kU, kClip>(p + base, g + base, m + base, numel - base, aligned, c);
   }
 }
 
@@ -256,9 +260,11 @@ template <typename TP> struct MultiShape {
                 "a CTA's part starts 16-byte aligned whenever the tensor does");
 };
 
-template <typename TP, typename TM>
+template <typename TP, typename TM, bool kClip>
 __global__ void __launch_bounds__(kThreads)
-lion_multi_tensor_kernel(const ChunkRecord* __restrict__ records, int64_t total_subs, LionConsts c) {
+lion_multi_tensor_kernel(const ChunkRecord* __restrict__ records, int64_t total_subs, LionConsts c,
+                         const float* __restrict__ clip) {
+  if constexpr (kClip) c.clip = __ldg(clip);
   for (int64_t sub = blockIdx.x; sub < total_subs; sub += gridDim.x) {
     using Shape = MultiShape<TP>;
     const uint4* rp = reinterpret_cast<const uint4*>(records + sub / Shape::kSubsPerChunk);
@@ -268,8 +274,8 @@ lion_multi_tensor_kernel(const ChunkRecord* __restrict__ records, int64_t total_
     memcpy(reinterpret_cast<char*>(&r) + 16, &hi, 16);
     const int64_t off = (sub % Shape::kSubsPerChunk) * static_cast<int64_t>(Shape::kSubElems);
     if (off >= r.remaining) continue;  // the tensor ended in an earlier part of this chunk
-    lion_chunk<TP, TM, Shape::kUnroll>(static_cast<TP*>(r.p) + off, static_cast<const TP*>(r.g) + off,
-                                      static_cast<TM*>(r.m) + off, r.remaining - off, all_aligned16(r.p, r.g, r.m), c);
+    lion_chunk<TP, TM, Shape::kUnroll, kClip>(static_cast<TP*>(r.p) + off, static_cast<const TP*>(r.g) + off,
+                                             static_cast<TM*>(r.m) + off, r.remaining - off, all_aligned16(r.p, r.g, r.m), c);
   }
 }
 
@@ -347,6 +353,7 @@ int make_consts(double lr, double beta1, double beta2, double wd, int p_dtype, i
   c->c_nlr = round_scalar(-lr, promoted);
   c->c_b2 = static_cast<float>(beta2);
   c->c_1mb2 = round_scalar(1.0 - beta2, promoted);
+  c->clip = 1.f;
   return FO_OK;
 }
 
@@ -367,12 +374,13 @@ int64_t one_wave_grid(int device, int64_t total_chunks) {
 }
 
 template <typename TP, typename TM>
-int launch_records_typed(const Plan& plan, const LionConsts& c, cudaStream_t stream) {
+int launch_records_typed(const Plan& plan, const LionConsts& c, const float* clip, cudaStream_t stream) {
   const int64_t total_subs = plan.total_chunks * MultiShape<TP>::kSubsPerChunk;
   // the kernel strides over its parts, so a grid cut at the launch limit still covers them all
   const int64_t grid = total_subs < 0x7fffffffll ? total_subs : 0x7fffffffll;
-  lion_multi_tensor_kernel<TP, TM><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
-      static_cast<const ChunkRecord*>(plan.d_blob), total_subs, c);
+  auto kernel = clip ? lion_multi_tensor_kernel<TP, TM, true> : lion_multi_tensor_kernel<TP, TM, false>;
+  kernel<<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(static_cast<const ChunkRecord*>(plan.d_blob), total_subs, c,
+                                                               clip);
   fo::g_launch_count.fetch_add(1, std::memory_order_relaxed);
   FO_CUDA_CHECK(cudaGetLastError());
   return FO_OK;
@@ -391,14 +399,15 @@ int launch_walk_typed(const Plan& plan, const LionConsts& c, cudaStream_t stream
 }
 
 template <typename TP, typename TM>
-int launch_single_typed(void* p, const void* g, void* m, int64_t numel, const LionConsts& c, int device,
+int launch_single_typed(void* p, const void* g, void* m, int64_t numel, const LionConsts& c, const float* clip,
                         cudaStream_t stream) {
   constexpr int kElems = kThreads * kVec * kSingleUnroll;
   const int64_t total_chunks = (numel + kElems - 1) / kElems;
   // the kernel strides over chunks, so a grid cut at the launch limit still covers them all
   const int64_t grid = total_chunks < 0x7fffffffll ? total_chunks : 0x7fffffffll;
-  lion_single_tensor_kernel<TP, TM><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
-      static_cast<TP*>(p), static_cast<const TP*>(g), static_cast<TM*>(m), numel, total_chunks, c);
+  auto kernel = clip ? lion_single_tensor_kernel<TP, TM, true> : lion_single_tensor_kernel<TP, TM, false>;
+  kernel<<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
+      static_cast<TP*>(p), static_cast<const TP*>(g), static_cast<TM*>(m), numel, total_chunks, c, clip);
   fo::g_launch_count.fetch_add(1, std::memory_order_relaxed);
   FO_CUDA_CHECK(cudaGetLastError());
   return FO_OK;
@@ -416,10 +425,11 @@ int launch_single_typed(void* p, const void* g, void* m, int64_t numel, const Li
   CASE(FO_F32, FO_F16, float, __half)
 
 // `plan.d_blob` holds chunk records.
-int launch_records(const Plan& plan, int p_dtype, int m_dtype, const LionConsts& c, cudaStream_t stream) {
+int launch_records(const Plan& plan, int p_dtype, int m_dtype, const LionConsts& c, const float* clip,
+                   cudaStream_t stream) {
   if (plan.total_chunks == 0) return FO_OK;
 #define FO_LION_CASE(PD, MD, TP, TM) \
-  if (p_dtype == PD && m_dtype == MD) return launch_records_typed<TP, TM>(plan, c, stream);
+  if (p_dtype == PD && m_dtype == MD) return launch_records_typed<TP, TM>(plan, c, clip, stream);
   FO_LION_DTYPE_CASES(FO_LION_CASE)
 #undef FO_LION_CASE
   return fo::fail(FO_ERR_INVALID_ARGUMENT, "unsupported Lion dtype combination p=%d m=%d", p_dtype, m_dtype);
@@ -436,9 +446,9 @@ int launch_walk(const Plan& plan, int p_dtype, int m_dtype, const LionConsts& c,
 }
 
 int launch_single(void* p, const void* g, void* m, int64_t numel, int p_dtype, int m_dtype, const LionConsts& c,
-                  int device, cudaStream_t stream) {
+                  const float* clip, cudaStream_t stream) {
 #define FO_LION_CASE(PD, MD, TP, TM) \
-  if (p_dtype == PD && m_dtype == MD) return launch_single_typed<TP, TM>(p, g, m, numel, c, device, stream);
+  if (p_dtype == PD && m_dtype == MD) return launch_single_typed<TP, TM>(p, g, m, numel, c, clip, stream);
   FO_LION_DTYPE_CASES(FO_LION_CASE)
 #undef FO_LION_CASE
   return fo::fail(FO_ERR_INVALID_ARGUMENT, "unsupported Lion dtype combination p=%d m=%d", p_dtype, m_dtype);
@@ -470,12 +480,10 @@ void build_records(void* const* params, const void* const* grads, void* const* e
 
 }  // namespace
 
-extern "C" int fo_lion_multi_tensor_step(void* const* params, const void* const* grads,
-                                         void* const* exp_avgs, const int64_t* numels, int n_tensors,
-                                         int p_dtype, int g_dtype, int m_dtype,
-                                         double lr, double beta1, double beta2, double weight_decay,
-                                         int device, void* stream) {
-  fo::clear_error();
+// `clip`: device address of the gradients' factor, or null for the step without one.
+static int multi_tensor_step(void* const* params, const void* const* grads, void* const* exp_avgs, const int64_t* numels,
+                             int n_tensors, int p_dtype, int g_dtype, int m_dtype, double lr, double beta1, double beta2,
+                             double weight_decay, const float* clip, int device, void* stream) {
   if (int rc = check_dtypes(p_dtype, g_dtype, m_dtype)) return rc;
   FO_REQUIRE(n_tensors >= 0, "n_tensors must be >= 0");
   if (n_tensors == 0) return FO_OK;
@@ -501,7 +509,7 @@ extern "C" int fo_lion_multi_tensor_step(void* const* params, const void* const*
   fo::DeviceGuard guard(device);
   FO_REQUIRE(guard.ok, "cannot make device %d current", device);
   if (n == 1)  // no table needed: the tensor travels in the kernel's arguments
-    return launch_single(ps[0], gs[0], ms[0], ns[0], p_dtype, m_dtype, c, device, static_cast<cudaStream_t>(stream));
+    return launch_single(ps[0], gs[0], ms[0], ns[0], p_dtype, m_dtype, c, clip, static_cast<cudaStream_t>(stream));
 
   // key: device, dtypes (the records hold byte addresses) and the raw list
   std::string key(reinterpret_cast<const char*>(&device), sizeof(device));
@@ -546,7 +554,28 @@ extern "C" int fo_lion_multi_tensor_step(void* const* params, const void* const*
     it = g_plans.emplace(std::move(key), plan).first;
   }
   it->second.last_use = ++g_plan_clock;
-  return launch_records(it->second, p_dtype, m_dtype, c, s);
+  return launch_records(it->second, p_dtype, m_dtype, c, clip, s);
+}
+
+extern "C" int fo_lion_multi_tensor_step(void* const* params, const void* const* grads,
+                                         void* const* exp_avgs, const int64_t* numels, int n_tensors,
+                                         int p_dtype, int g_dtype, int m_dtype,
+                                         double lr, double beta1, double beta2, double weight_decay,
+                                         int device, void* stream) {
+  fo::clear_error();
+  return multi_tensor_step(params, grads, exp_avgs, numels, n_tensors, p_dtype, g_dtype, m_dtype, lr, beta1, beta2,
+                           weight_decay, nullptr, device, stream);
+}
+
+extern "C" int fo_lion_multi_tensor_step_clipped(void* const* params, const void* const* grads,
+                                                 void* const* exp_avgs, const int64_t* numels, int n_tensors,
+                                                 int p_dtype, int g_dtype, int m_dtype,
+                                                 double lr, double beta1, double beta2, double weight_decay,
+                                                 const float* clip, int device, void* stream) {
+  fo::clear_error();
+  FO_REQUIRE(clip != nullptr, "null clipping factor");
+  return multi_tensor_step(params, grads, exp_avgs, numels, n_tensors, p_dtype, g_dtype, m_dtype, lr, beta1, beta2,
+                           weight_decay, clip, device, stream);
 }
 
 extern "C" int fo_lion_clear_cache(void) {
@@ -556,11 +585,9 @@ extern "C" int fo_lion_clear_cache(void) {
   return FO_OK;
 }
 
-extern "C" int fo_lion_update(void* param, const void* grad, void* exp_avg, int64_t numel,
-                              int p_dtype, int g_dtype, int m_dtype,
-                              double lr, double beta1, double beta2, double weight_decay,
+static int single_tensor_step(void* param, const void* grad, void* exp_avg, int64_t numel, int p_dtype, int g_dtype,
+                              int m_dtype, double lr, double beta1, double beta2, double weight_decay, const float* clip,
                               int device, void* stream) {
-  fo::clear_error();
   if (int rc = check_dtypes(p_dtype, g_dtype, m_dtype)) return rc;
   FO_REQUIRE(numel >= 0, "negative numel");
   if (numel == 0) return FO_OK;
@@ -569,7 +596,30 @@ extern "C" int fo_lion_update(void* param, const void* grad, void* exp_avg, int6
   if (int rc = make_consts(lr, beta1, beta2, weight_decay, p_dtype, m_dtype, &c)) return rc;
   fo::DeviceGuard guard(device);
   FO_REQUIRE(guard.ok, "cannot make device %d current", device);
-  return launch_single(param, grad, exp_avg, numel, p_dtype, m_dtype, c, device, static_cast<cudaStream_t>(stream));
+  return launch_single(param, grad, exp_avg, numel, p_dtype, m_dtype, c, clip, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int fo_lion_update(void* param, const void* grad, void* exp_avg, int64_t numel,
+                              int p_dtype, int g_dtype, int m_dtype,
+                              double lr, double beta1, double beta2, double weight_decay,
+                              int device, void* stream) {
+  fo::clear_error();
+  return single_tensor_step(param, grad, exp_avg, numel, p_dtype, g_dtype, m_dtype, lr, beta1, beta2, weight_decay, nullptr,
+                            device, stream);
+}
+
+static int flat_step(void* param, const void* grad, void* exp_avg_shard, int64_t begin, int64_t end, int p_dtype, int g_dtype,
+                     int m_dtype, double lr, double beta1, double beta2, double weight_decay, const float* clip, int device,
+                     void* stream) {
+  if (int rc = check_dtypes(p_dtype, g_dtype, m_dtype)) return rc;
+  FO_REQUIRE(begin >= 0 && end >= begin, "bad shard range [%lld, %lld)", (long long)begin, (long long)end);
+  if (end == begin) return FO_OK;
+  FO_REQUIRE(param && grad && exp_avg_shard, "null pointer");
+  const int64_t esz = (p_dtype == FO_F32) ? 4 : 2;
+  void* p = static_cast<char*>(param) + begin * esz;
+  const void* g = static_cast<const char*>(grad) + begin * esz;
+  return single_tensor_step(p, g, exp_avg_shard, end - begin, p_dtype, g_dtype, m_dtype, lr, beta1, beta2, weight_decay, clip,
+                            device, stream);
 }
 
 extern "C" int fo_lion_flat_step(void* param, const void* grad, void* exp_avg_shard,
@@ -578,15 +628,19 @@ extern "C" int fo_lion_flat_step(void* param, const void* grad, void* exp_avg_sh
                                  double lr, double beta1, double beta2, double weight_decay,
                                  int device, void* stream) {
   fo::clear_error();
-  if (int rc = check_dtypes(p_dtype, g_dtype, m_dtype)) return rc;
-  FO_REQUIRE(begin >= 0 && end >= begin, "bad shard range [%lld, %lld)", (long long)begin, (long long)end);
-  if (end == begin) return FO_OK;
-  FO_REQUIRE(param && grad && exp_avg_shard, "null pointer");
-  const int64_t esz = (p_dtype == FO_F32) ? 4 : 2;
-  void* p = static_cast<char*>(param) + begin * esz;
-  const void* g = static_cast<const char*>(grad) + begin * esz;
-  return fo_lion_update(p, g, exp_avg_shard, end - begin, p_dtype, g_dtype, m_dtype, lr, beta1, beta2,
-                        weight_decay, device, stream);
+  return flat_step(param, grad, exp_avg_shard, begin, end, p_dtype, g_dtype, m_dtype, lr, beta1, beta2, weight_decay, nullptr,
+                   device, stream);
+}
+
+extern "C" int fo_lion_flat_step_clipped(void* param, const void* grad, void* exp_avg_shard,
+                                         int64_t begin, int64_t end,
+                                         int p_dtype, int g_dtype, int m_dtype,
+                                         double lr, double beta1, double beta2, double weight_decay,
+                                         const float* clip, int device, void* stream) {
+  fo::clear_error();
+  FO_REQUIRE(clip != nullptr, "null clipping factor");
+  return flat_step(param, grad, exp_avg_shard, begin, end, p_dtype, g_dtype, m_dtype, lr, beta1, beta2, weight_decay, clip,
+                   device, stream);
 }
 
 // ---- allocation-free variant -----------------------------------------------------------------
@@ -723,10 +777,11 @@ struct PeerList {
 constexpr int kPushUnroll = 1;
 constexpr int kPushElems = kThreads * kVec * kPushUnroll;
 
-template <typename TP, typename TM>
+template <typename TP, typename TM, bool kClip>
 __global__ void __launch_bounds__(kThreads)
 lion_flat_push_kernel(TP* __restrict__ p_local, const TP* __restrict__ g, TM* __restrict__ m_shard,
-                      int64_t begin, int64_t numel, PeerList peers, LionConsts c) {
+                      int64_t begin, int64_t numel, PeerList peers, LionConsts c, const float* __restrict__ clip) {
+  if constexpr (kClip) c.clip = __ldg(clip);
   // p_local, g and the peers' bases address element 0 of the flat buffers; m_shard addresses the
   // momentum of element `begin`.
   const int64_t total_chunks = (numel + kPushElems - 1) / kPushElems;
@@ -756,7 +811,7 @@ lion_flat_push_kernel(TP* __restrict__ p_local, const TP* __restrict__ g, TM* __
       }
 #pragma unroll
       for (int u = 0; u < kPushUnroll; ++u) {
-        lion_group<TP, TM>(pv[u], gv[u], mv[u], c);
+        lion_group<TP, TM, kClip>(pv[u], gv[u], mv[u], c);
         const int off = (u * kThreads + threadIdx.x) * kVec;
         store_group(p + off, pv[u]);
         store_group(m + off, mv[u]);
@@ -776,7 +831,7 @@ lion_flat_push_kernel(TP* __restrict__ p_local, const TP* __restrict__ g, TM* __
       for (int i = threadIdx.x; i < n; i += kThreads) {
         TP pe = p[i];
         TM me = m[i];
-        lion_element<TP, TM>(pe, gg[i], me, c);
+        lion_element<TP, TM, kClip>(pe, gg[i], me, c);
         p[i] = pe;
         m[i] = me;
 #pragma unroll
@@ -789,12 +844,13 @@ lion_flat_push_kernel(TP* __restrict__ p_local, const TP* __restrict__ g, TM* __
 
 template <typename TP, typename TM>
 int launch_push(void* p, const void* g, void* m, int64_t begin, int64_t numel, const PeerList& peers,
-                const LionConsts& c, int device, cudaStream_t stream) {
+                const LionConsts& c, const float* clip, cudaStream_t stream) {
   const int64_t total_chunks = (numel + kPushElems - 1) / kPushElems;
   // the kernel strides over chunks, so a grid cut at the launch limit still covers them all
   const int64_t grid = total_chunks < 0x7fffffffll ? total_chunks : 0x7fffffffll;
-  lion_flat_push_kernel<TP, TM><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
-      static_cast<TP*>(p), static_cast<const TP*>(g), static_cast<TM*>(m), begin, numel, peers, c);
+  auto kernel = clip ? lion_flat_push_kernel<TP, TM, true> : lion_flat_push_kernel<TP, TM, false>;
+  kernel<<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(
+      static_cast<TP*>(p), static_cast<const TP*>(g), static_cast<TM*>(m), begin, numel, peers, c, clip);
   fo::g_launch_count.fetch_add(1, std::memory_order_relaxed);
   FO_CUDA_CHECK(cudaGetLastError());
   return FO_OK;
@@ -802,13 +858,9 @@ int launch_push(void* p, const void* g, void* m, int64_t begin, int64_t numel, c
 
 }  // namespace
 
-extern "C" int fo_lion_flat_step_push(void* param, const void* grad, void* exp_avg_shard,
-                                      int64_t begin, int64_t end,
-                                      void* const* peer_params, int n_peers,
-                                      int p_dtype, int g_dtype, int m_dtype,
-                                      double lr, double beta1, double beta2, double weight_decay,
-                                      int device, void* stream) {
-  fo::clear_error();
+static int flat_step_push(void* param, const void* grad, void* exp_avg_shard, int64_t begin, int64_t end,
+                          void* const* peer_params, int n_peers, int p_dtype, int g_dtype, int m_dtype, double lr,
+                          double beta1, double beta2, double weight_decay, const float* clip, int device, void* stream) {
   if (int rc = check_dtypes(p_dtype, g_dtype, m_dtype)) return rc;
   FO_REQUIRE(begin >= 0 && end >= begin, "bad shard range [%lld, %lld)", (long long)begin, (long long)end);
   FO_REQUIRE(n_peers >= 0 && n_peers <= kMaxPeers, "n_peers must be in [0, %d] (got %d)", kMaxPeers, n_peers);
@@ -830,7 +882,7 @@ extern "C" int fo_lion_flat_step_push(void* param, const void* grad, void* exp_a
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int64_t n = end - begin;
 #define FO_LION_PUSH_CASE(PD, MD, TP, TM) \
-  if (p_dtype == PD && m_dtype == MD) return launch_push<TP, TM>(param, grad, exp_avg_shard, begin, n, peers, c, device, s);
+  if (p_dtype == PD && m_dtype == MD) return launch_push<TP, TM>(param, grad, exp_avg_shard, begin, n, peers, c, clip, s);
   FO_LION_PUSH_CASE(FO_BF16, FO_BF16, __nv_bfloat16, __nv_bfloat16)
   FO_LION_PUSH_CASE(FO_BF16, FO_F32, __nv_bfloat16, float)
   FO_LION_PUSH_CASE(FO_F16, FO_F16, __half, __half)
@@ -839,4 +891,27 @@ extern "C" int fo_lion_flat_step_push(void* param, const void* grad, void* exp_a
   FO_LION_PUSH_CASE(FO_F32, FO_BF16, float, __nv_bfloat16)
 #undef FO_LION_PUSH_CASE
   return fo::fail(FO_ERR_UNSUPPORTED, "no fused-gather Lion kernel for dtypes p=%d m=%d", p_dtype, m_dtype);
+}
+
+extern "C" int fo_lion_flat_step_push(void* param, const void* grad, void* exp_avg_shard,
+                                      int64_t begin, int64_t end,
+                                      void* const* peer_params, int n_peers,
+                                      int p_dtype, int g_dtype, int m_dtype,
+                                      double lr, double beta1, double beta2, double weight_decay,
+                                      int device, void* stream) {
+  fo::clear_error();
+  return flat_step_push(param, grad, exp_avg_shard, begin, end, peer_params, n_peers, p_dtype, g_dtype, m_dtype, lr, beta1,
+                        beta2, weight_decay, nullptr, device, stream);
+}
+
+extern "C" int fo_lion_flat_step_push_clipped(void* param, const void* grad, void* exp_avg_shard,
+                                              int64_t begin, int64_t end,
+                                              void* const* peer_params, int n_peers,
+                                              int p_dtype, int g_dtype, int m_dtype,
+                                              double lr, double beta1, double beta2, double weight_decay,
+                                              const float* clip, int device, void* stream) {
+  fo::clear_error();
+  FO_REQUIRE(clip != nullptr, "null clipping factor");
+  return flat_step_push(param, grad, exp_avg_shard, begin, end, peer_params, n_peers, p_dtype, g_dtype, m_dtype, lr, beta1,
+                        beta2, weight_decay, clip, device, stream);
 }

@@ -1,0 +1,96 @@
+"""The 2-norm over the gradients of a whole model, on the device.
+
+`grad_norm` is the plain call; `Lion(..., max_grad_norm=c)` makes the same one before its step and
+hands the clipping factor to the step's kernel in device memory, so that the gradients are never
+rewritten and nothing waits for the host.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Iterable, List, Optional, Tuple
+
+import torch
+from torch import Tensor
+
+from .. import _lib
+
+
+def is_dense(t: Tensor) -> bool:
+    """True when the tensor's elements fill one gap-free block of memory in some order
+    (the reference's `is_non_overlapping_and_dense`, fast_ops/lion/lion_update.cu:109-112)."""
+    if t.is_contiguous() or t.numel() == 0:
+        return True
+    strides = sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1)
+    expect = 1
+    for st, sz in strides:
+        if st != expect:
+            return False
+        expect *= sz
+    return True
+
+
+class GradList:
+    """ctypes image of the gradients of one norm call."""
+
+    def __init__(self, grads: List[Tensor]):
+        if not grads:
+            raise RuntimeError("grad_norm needs at least one tensor")
+        for g in grads:
+            if not isinstance(g, Tensor) or g.layout != torch.strided:
+                raise RuntimeError("gradients must be dense tensors")
+            if not g.is_cuda:
+                raise RuntimeError("fast_ops_b200 grad_norm needs CUDA tensors (there is no CPU path)")
+        device = grads[0].device
+        for g in grads:
+            if g.device != device:
+                raise RuntimeError("all gradients must be on one device")
+            if not is_dense(g):
+                raise RuntimeError("expected tensor to be contiguous")
+        n = len(grads)
+        self.n, self.device, self.device_index = n, device, device.index
+        self.ptrs = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
+        self.numels = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
+        self.dtypes = (ctypes.c_int * n)(*[_lib.dtype_code(g.dtype) for g in grads])
+        self.doubles = int(_lib.load().fo_grad_norm_workspace(n))
+
+    def launch(self, max_norm: float, sumsq: Optional[Tensor] = None) -> Tensor:
+        """(norm, clipping factor) as two floats on the device; `sumsq`, if given, receives the sum of
+        squares as a double.  Workspace and result are allocated by the call, so that calls on
+        different streams or in different graphs share nothing."""
+        workspace = torch.empty(self.doubles, dtype=torch.float64, device=self.device)
+        result = torch.empty(2, dtype=torch.float32, device=self.device)
+        _lib.check(_lib.load().fo_grad_norm(
+            self.ptrs, self.numels, self.dtypes, self.n, max_norm, workspace.data_ptr(),
+            None if sumsq is None else sumsq.data_ptr(), result.data_ptr(), self.device_index,
+            _lib.current_stream_ptr(self.device_index)))
+        return result
+
+
+def grad_norm(grads: Iterable[Tensor]) -> Tensor:
+    """The 2-norm of all elements of `grads` together, a 0-d fp32 tensor on their device.
+
+    The tensors may be fp16, bf16 and fp32, mixed as they come, of any size, each dense in memory and
+    all on one CUDA device (violations raise RuntimeError, an empty list too).  Sums are formed in
+    double in a fixed order: the same gradients give the same bits, and squares that leave the range
+    of fp32 count.  Non-finite gradients give a non-finite norm.  Not differentiable.  The call
+    does not wait for the device and may be captured into a CUDA graph.
+    """
+    if isinstance(grads, Tensor):
+        grads = [grads]
+    with torch.no_grad():
+        return GradList(list(grads)).launch(float("inf"))[0]
+
+
+def finish_norm(sumsq: Tensor, max_norm: float) -> Tensor:
+    """(norm, clipping factor) from a sum of squares (a double on the device)."""
+    result = torch.empty(2, dtype=torch.float32, device=sumsq.device)
+    _lib.check(_lib.load().fo_grad_norm_finish(sumsq.data_ptr(), max_norm, result.data_ptr(), sumsq.device.index,
+                                               _lib.current_stream_ptr(sumsq.device.index)))
+    return result
+
+
+def shard_sumsq(flat_g: Tensor, begin: int, end: int) -> Tensor:
+    """Sum of squares of elements [begin, end) of a flat gradient buffer, a one-element double."""
+    sumsq = torch.empty(1, dtype=torch.float64, device=flat_g.device)
+    GradList([flat_g[begin:end]]).launch(float("inf"), sumsq)
+    return sumsq

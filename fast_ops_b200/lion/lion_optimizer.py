@@ -19,6 +19,11 @@ Keyword-only extensions:
   reduce_gradients with process_group: step() first averages the flat gradient buffer across
                    the ranks with one reduce-scatter into this rank's slice (otherwise the caller
                    is expected to have reduced the gradients already).
+  max_grad_norm    step() first takes the 2-norm over the gradients of all parameters (over all
+                   ranks' slices with process_group) and applies every gradient times
+                   min(1, max_grad_norm / (norm + 1e-6)), rounded to the gradient's type once, as if
+                   it had been clipped in memory.  The factor stays on the device and the stored
+                   gradients are left as they are.  `grad_norm` is the norm of the latest step.
 """
 from __future__ import annotations
 
@@ -30,6 +35,7 @@ from torch import Tensor
 from torch.optim.optimizer import Optimizer
 
 from .. import _lib
+from .grad_norm import GradList, finish_norm, is_dense as _is_dense, shard_sumsq
 from .zero1 import FlatLayout
 
 
@@ -45,20 +51,6 @@ def lion_update(param: Tensor, grad: Tensor, exp_avg: Tensor, lr: float, beta1: 
         _lib.dtype_code(param.dtype), _lib.dtype_code(grad.dtype), _lib.dtype_code(exp_avg.dtype),
         float(lr), float(beta1), float(beta2), float(weight_decay), param.device.index,
         _lib.current_stream_ptr(param.device)))
-
-
-def _is_dense(t: Tensor) -> bool:
-    """True when the tensor's elements fill one gap-free block of memory in some order
-    (the reference's `is_non_overlapping_and_dense`, fast_ops/lion/lion_update.cu:109-112)."""
-    if t.is_contiguous() or t.numel() == 0:
-        return True
-    strides = sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1)
-    expect = 1
-    for st, sz in strides:
-        if st != expect:
-            return False
-        expect *= sz
-    return True
 
 
 def _check_triple(param: Tensor, grad: Tensor, exp_avg: Tensor) -> None:
@@ -78,26 +70,32 @@ def _check_triple(param: Tensor, grad: Tensor, exp_avg: Tensor) -> None:
 
 
 def _flat_step_push(p: Tensor, g: Tensor, m_shard: Tensor, begin: int, end: int, peer_ptrs, lr: float, betas,
-                    wd: float) -> None:
+                    wd: float, clip: Optional[Tensor] = None) -> None:
     """Lion step on [begin, end) that also stores the result into the peers' flat buffers
-    (C-ABI fo_lion_flat_step_push).  `peer_ptrs`: device addresses of the peers' element 0."""
+    (C-ABI fo_lion_flat_step_push).  `peer_ptrs`: device addresses of the peers' element 0; `clip`: a
+    device float that multiplies the gradients."""
     lib = _lib.load()
     n = len(peer_ptrs)
     arr = (ctypes.c_void_p * max(n, 1))(*peer_ptrs)
-    _lib.check(lib.fo_lion_flat_step_push(
+    entry, extra = (lib.fo_lion_flat_step_push, ()) if clip is None else (
+        lib.fo_lion_flat_step_push_clipped, (clip.data_ptr(),))
+    _lib.check(entry(
         p.data_ptr(), g.data_ptr(), m_shard.data_ptr(), begin, end, arr, n,
         _lib.dtype_code(p.dtype), _lib.dtype_code(g.dtype), _lib.dtype_code(m_shard.dtype),
-        float(lr), float(betas[0]), float(betas[1]), float(wd), p.device.index,
+        float(lr), float(betas[0]), float(betas[1]), float(wd), *extra, p.device.index,
         _lib.current_stream_ptr(p.device)))
 
 
-def _flat_step(p: Tensor, g: Tensor, m_shard: Tensor, begin: int, end: int, lr: float, betas, wd: float) -> None:
-    """Lion step on elements [begin, end) of the flat buffers (C-ABI fo_lion_flat_step)."""
+def _flat_step(p: Tensor, g: Tensor, m_shard: Tensor, begin: int, end: int, lr: float, betas, wd: float,
+               clip: Optional[Tensor] = None) -> None:
+    """Lion step on elements [begin, end) of the flat buffers (C-ABI fo_lion_flat_step); `clip`: a device
+    float that multiplies the gradients."""
     lib = _lib.load()
-    _lib.check(lib.fo_lion_flat_step(
+    entry, extra = (lib.fo_lion_flat_step, ()) if clip is None else (lib.fo_lion_flat_step_clipped, (clip.data_ptr(),))
+    _lib.check(entry(
         p.data_ptr(), g.data_ptr(), m_shard.data_ptr(), begin, end,
         _lib.dtype_code(p.dtype), _lib.dtype_code(g.dtype), _lib.dtype_code(m_shard.dtype),
-        float(lr), float(betas[0]), float(betas[1]), float(wd), p.device.index,
+        float(lr), float(betas[0]), float(betas[1]), float(wd), *extra, p.device.index,
         _lib.current_stream_ptr(p.device)))
 
 
@@ -120,17 +118,25 @@ class Lion(Optimizer):
 
     def __init__(self, params: Iterable, lr: float = 1e-4, betas: Tuple[float, float] = (0.9, 0.99),
                  weight_decay: float = 0.0, *, momentum_dtype: Optional[torch.dtype] = None,
-                 process_group=None, fused_gather: bool = False, reduce_gradients: bool = False) -> None:
+                 process_group=None, fused_gather: bool = False, reduce_gradients: bool = False,
+                 max_grad_norm: Optional[float] = None) -> None:
         if lr <= 0:
             raise RuntimeError(f"expected positive LR, got {lr}")
         if not all(0 <= beta <= 1 for beta in betas):
             raise RuntimeError(f"betas must be between 0 and 1. got {betas}")
         if momentum_dtype not in (None, torch.float16, torch.bfloat16, torch.float32):
             raise RuntimeError(f"unsupported momentum dtype {momentum_dtype}")
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise RuntimeError(f"max_grad_norm must be positive, got {max_grad_norm}")
         defaults = {"lr": lr, "betas": betas, "weight_decay": weight_decay}
         super().__init__(params, defaults)
         self._momentum_dtype = momentum_dtype
         self._lists: Dict[int, tuple] = {}  # group index -> (address signature, prepared launches)
+        self.max_grad_norm = max_grad_norm
+        #: 0-d fp32 tensor: the norm of all gradients at the latest step, before clipping; None before the
+        #: first one and without max_grad_norm
+        self.grad_norm: Optional[Tensor] = None
+        self._grad_list: Optional[Tuple[list, Optional[GradList]]] = None
         self._pg = process_group
         self._zero = None
         if fused_gather and process_group is None:
@@ -180,27 +186,57 @@ class Lion(Optimizer):
             self._zero.step()
             return
         lib = _lib.load()
+        clip = self._clip_factor() if self.max_grad_norm is not None else None
         for gi, group in enumerate(self.param_groups):
-            # A training loop presents the same tensors step after step: while no parameter or
-            # gradient address has changed, the checks and the pointer arrays of the last step stand.
-            sig = self._signature(group)
-            cached = self._lists.get(gi)
-            if cached is None or cached[0] != sig:
-                cached = (sig, self._prepare_group(gi, group))
-                self._lists[gi] = cached
             lr = float(group["lr"])
             weight_decay = float(group["weight_decay"])
             beta1, beta2 = (float(b) for b in group["betas"])
-            for tl in cached[1]:
-                _lib.check(lib.fo_lion_multi_tensor_step(
-                    tl.params, tl.grads, tl.moms, tl.numels, tl.n, tl.p_code, tl.p_code, tl.m_code,
-                    lr, beta1, beta2, weight_decay, tl.device_index, _lib.current_stream_ptr(tl.device_index)))
+            # with clipping the lists have just been looked up, for the norm
+            for tl in self._group_lists(gi, group) if clip is None else self._lists[gi][1]:
+                args = (tl.params, tl.grads, tl.moms, tl.numels, tl.n, tl.p_code, tl.p_code, tl.m_code,
+                        lr, beta1, beta2, weight_decay)
+                where = (tl.device_index, _lib.current_stream_ptr(tl.device_index))
+                if clip is None:
+                    _lib.check(lib.fo_lion_multi_tensor_step(*args, *where))
+                else:
+                    _lib.check(lib.fo_lion_multi_tensor_step_clipped(*args, clip.data_ptr(), *where))
+
+    def _group_lists(self, gi: int, group) -> list:
+        """The group's prepared launches.  A training loop presents the same tensors step after step:
+        while no parameter or gradient address has changed, the checks and the pointer arrays of the
+        last step stand."""
+        sig = self._signature(group)
+        cached = self._lists.get(gi)
+        if cached is None or cached[0] != sig:
+            cached = (sig, self._prepare_group(gi, group))
+            self._lists[gi] = cached
+        return cached[1]
+
+    def _clip_factor(self) -> Optional[Tensor]:
+        """Launches the norm over the gradients of all groups; returns the clipping factor, a device
+        float, or None when no parameter has a gradient."""
+        max_norm = float(self.max_grad_norm)
+        if not max_norm > 0:
+            raise RuntimeError(f"max_grad_norm must be positive, got {max_norm}")
+        lists = [tl for gi, group in enumerate(self.param_groups) for tl in self._group_lists(gi, group)]
+        if self._grad_list is None or len(self._grad_list[0]) != len(lists) or any(
+                a is not b for a, b in zip(self._grad_list[0], lists)):
+            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            self._grad_list = (lists, GradList(grads) if grads else None)
+        grad_list = self._grad_list[1]
+        if grad_list is None:
+            self.grad_norm = None
+            return None
+        result = grad_list.launch(max_norm)
+        self.grad_norm = result[0]
+        return result[1]
 
     def load_state_dict(self, state_dict) -> None:
         """As torch.optim.Optimizer.load_state_dict; in process_group mode the loaded momentum
         (this rank's slices, as state_dict() saved them) is copied back into the rank's shard."""
         super().load_state_dict(state_dict)
         self._lists.clear()  # the momentum tensors are new objects
+        self._grad_list = None
         if self._zero is not None:
             self._zero.adopt_loaded_state()
 
@@ -276,6 +312,8 @@ class _Zero1State:
             _, s0, n = self.layout.tensor_slice_in_shard(i, self.rank)
             opt.state[p]["exp_avg"] = self.m_shard[s0:s0 + n]
         self.flat_step_fn = _flat_step
+        # the two halves of the clipping factor, around the all-reduce of the sum of squares
+        self.sumsq_fn, self.finish_norm_fn = shard_sumsq, finish_norm
 
     def adopt_loaded_state(self) -> None:
         """After Optimizer.load_state_dict: state[p]["exp_avg"] holds fresh tensors; copy them
@@ -301,6 +339,21 @@ class _Zero1State:
         else:
             dist.reduce_scatter_tensor(shard, self.flat_g, op=dist.ReduceOp.AVG, group=self.group)
 
+    def _clip_factor(self) -> Tensor:
+        """Sum of squares of this rank's slice, added up over the ranks (every element of the flat
+        gradient lies in one slice), then the factor: the same on all ranks."""
+        import torch.distributed as dist
+
+        max_norm = float(self.opt.max_grad_norm)
+        if not max_norm > 0:
+            raise RuntimeError(f"max_grad_norm must be positive, got {max_norm}")
+        sumsq = self.sumsq_fn(self.flat_g, self.begin, self.end)
+        if self.world > 1:
+            dist.all_reduce(sumsq, group=self.group)
+        result = self.finish_norm_fn(sumsq, max_norm)
+        self.opt.grad_norm = result[0]
+        return result[1]
+
     @torch.no_grad()
     def step(self) -> None:
         import torch.distributed as dist
@@ -314,15 +367,16 @@ class _Zero1State:
         if self.reduce_gradients and self.world > 1:
             self._average_gradients()
         group = self.opt.param_groups[0]
+        clip = {} if self.opt.max_grad_norm is None else {"clip": self._clip_factor()}
         if self.symm is not None:
             # ranks meet before any of them overwrites a peer's weights, and again before any of
             # them reads the gathered result (device-side barriers on the current stream)
             self.symm.barrier(channel=0)
             _flat_step_push(self.flat_p, self.flat_g, self.m_shard, self.begin, self.end, self.peer_ptrs,
-                            group["lr"], group["betas"], group["weight_decay"])
+                            group["lr"], group["betas"], group["weight_decay"], **clip)
             self.symm.barrier(channel=1)
             return
         self.flat_step_fn(self.flat_p, self.flat_g, self.m_shard, self.begin, self.end, group["lr"],
-                          group["betas"], group["weight_decay"])
+                          group["betas"], group["weight_decay"], **clip)
         if self.world > 1:
             dist.all_gather_into_tensor(self.flat_p, self.flat_p[self.begin:self.end], group=self.group)

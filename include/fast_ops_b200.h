@@ -250,6 +250,55 @@ int fo_lion_multi_tensor_step_noalloc(void* const* params, const void* const* gr
                                       double lr, double beta1, double beta2, double weight_decay,
                                       int device, void* stream);
 
+/*
+ * fo_lion_multi_tensor_step, fo_lion_flat_step and fo_lion_flat_step_push with the gradients multiplied
+ * by *clip (a device float, read when the kernel runs; fo_grad_norm writes one) and rounded to their
+ * type once, as if they had been scaled in memory before the step.  The gradients themselves are not written.  No
+ * counterpart in the reference.
+ */
+int fo_lion_multi_tensor_step_clipped(void* const* params, const void* const* grads,
+                                      void* const* exp_avgs, const int64_t* numels, int n_tensors,
+                                      int p_dtype, int g_dtype, int m_dtype,
+                                      double lr, double beta1, double beta2, double weight_decay,
+                                      const float* clip, int device, void* stream);
+int fo_lion_flat_step_clipped(void* param, const void* grad, void* exp_avg_shard,
+                              int64_t begin, int64_t end,
+                              int p_dtype, int g_dtype, int m_dtype,
+                              double lr, double beta1, double beta2, double weight_decay,
+                              const float* clip, int device, void* stream);
+int fo_lion_flat_step_push_clipped(void* param, const void* grad, void* exp_avg_shard,
+                                   int64_t begin, int64_t end,
+                                   void* const* peer_params, int n_peers,
+                                   int p_dtype, int g_dtype, int m_dtype,
+                                   double lr, double beta1, double beta2, double weight_decay,
+                                   const float* clip, int device, void* stream);
+
+/*
+ * The 2-norm over all elements of a list of gradients and the factor that clips them to a norm:
+ *   norm = sqrt(sum_t sum_i g_t[i]^2),  coef = min(1, max_norm / (norm + 1e-6))
+ * Sums are formed in double, in an order that does not change from run to run; elements of any finite
+ * size count (fp32 values whose squares overflow included).  An infinite or NaN gradient gives an
+ * infinite or NaN norm.  The reference has no counterpart.
+ *
+ *   grads, numels, dtypes : HOST arrays of n_tensors device pointers, element counts and element
+ *                types (FO_F16, FO_BF16, FO_F32, mixed as they come); each tensor dense.  The list
+ *                travels in the kernel's arguments: nothing is cached or allocated, and a call may be
+ *                captured into a CUDA graph without one outside before it.
+ *   max_norm   : non-negative, may be infinite (coef is then 1 unless the norm is infinite or NaN).
+ *   workspace  : device memory of fo_grad_norm_workspace(n_tensors) doubles, 8-byte aligned, not
+ *                shared with a call that may run at the same time; contents on entry do not matter.
+ *   sumsq      : device double that receives the sum of squares, or NULL.
+ *   norm_coef  : two device floats that receive norm and coef, or NULL.
+ */
+int fo_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int n_tensors,
+                 double max_norm, double* workspace, double* sumsq, float* norm_coef,
+                 int device, void* stream);
+int64_t fo_grad_norm_workspace(int n_tensors);
+
+/* Norm and coef, as fo_grad_norm writes them, from a sum of squares in device memory (one that has
+ * been added up over the ranks of a sharded gradient). */
+int fo_grad_norm_finish(const double* sumsq, double max_norm, float* norm_coef, int device, void* stream);
+
 /* Drops the cached tensor tables of fo_lion_multi_tensor_step (all devices). */
 int fo_lion_clear_cache(void);
 
