@@ -6,6 +6,7 @@
 #include <cstring>
 
 #include "flash_attn_bwd.cuh"
+#include "flash_attn_host.h"
 #include "fo_host.h"
 #include "fo_tma.h"
 
@@ -76,19 +77,6 @@ attn_bwd_finish_dq_kernel(const float* __restrict__ dq_accum, uint16_t* __restri
   *reinterpret_cast<uint4*>(dq + b * q_sb + h * q_sh + row * q_ss + d0) = v;
 }
 
-template <int D, bool kBf16, int kExt, int kMma = D>
-int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
-               const CUtensorMap& tdq, const fo::AttnBwdParams& prm, cudaStream_t stream) {
-  dim3 grid((prm.Sk + fo::kBlockN - 1) / fo::kBlockN, prm.B * prm.H);
-  auto kernel = fo::attn_bwd_kernel<D, kBf16, kExt, kMma>;
-  constexpr int smem = fo::BwdConfig<D, kExt>::kSmemBytes;
-  FO_CUDA_CHECK((fo::ensure_dynamic_smem<fo::attn_bwd_kernel<D, kBf16, kExt, kMma>>(smem, prm.device)));
-  kernel<<<grid, fo::BwdConfig<D, kExt>::kThreads, smem, stream>>>(tq, tk, tv, tdo, tdq, prm);
-  fo::g_launch_count.fetch_add(1, std::memory_order_relaxed);
-  FO_CUDA_CHECK(cudaGetLastError());
-  return FO_OK;
-}
-
 int check_out_strides(const int64_t s[3], const char* name) {
   for (int i = 0; i < 3; ++i)
     FO_REQUIRE(s[i] >= 0 && s[i] % 8 == 0, "%s: strides must be non-negative multiples of 8 elements", name);
@@ -97,20 +85,15 @@ int check_out_strides(const int64_t s[3], const char* name) {
 
 }  // namespace
 
-namespace fo {
-int make_attn_extras(AttnExtras* ex, const void* bias, const int64_t* bias_strides, int bias_dtype, int dtype,
-                     float dropout_p, uint64_t rng_seed, uint64_t rng_offset);  // flash_attn_fwd.cu
-}
-
-static int attn_bwd_impl(const void* q, const void* k, const void* v, const void* o, const void* dout,
-                         const float* lse, void* dq, void* dk, void* dv, float* dq_accum, float* delta,
-                         int B, int H, int Sq, int Sk, int D,
-                         const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
-                         const int64_t o_strides[3], const int64_t do_strides[3],
-                         const int64_t dq_strides[3], const int64_t dk_strides[3],
-                         const int64_t dv_strides[3],
-                         int dtype, int causal, float softmax_scale, const fo::AttnExtras* ex, int device,
-                         void* stream) {
+int fo::attn_bwd_impl(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                      const float* lse, void* dq, void* dk, void* dv, float* dq_accum, float* delta,
+                      int B, int H, int Sq, int Sk, int D,
+                      const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                      const int64_t o_strides[3], const int64_t do_strides[3],
+                      const int64_t dq_strides[3], const int64_t dk_strides[3],
+                      const int64_t dv_strides[3],
+                      int dtype, int causal, float softmax_scale, const fo::AttnExtras* ex,
+                      const fo::RelArgs* rel, int device, void* stream) {
   FO_REQUIRE(q && k && v && o && dout && lse && dq && dk && dv && dq_accum && delta, "null pointer");
   FO_REQUIRE(q_strides && k_strides && v_strides && o_strides && do_strides && dq_strides && dk_strides && dv_strides,
              "null stride array");
@@ -186,19 +169,23 @@ static int attn_bwd_impl(const void* q, const void* k, const void* v, const void
   prm.ex.drop_rescale = 1.f;
   const bool ext = ex != nullptr && (ex->bias != nullptr || ex->dropout);
   if (ext) prm.ex = *ex;
+  std::memset(&prm.rel, 0, sizeof(prm.rel));
+  if (rel) prm.rel = rel->bias;
   int rc;
   const int bias_mode = !ext || prm.ex.bias == nullptr ? 0 : prm.ex.bias_stride_q == 0 ? fo::kBwdVecBias : fo::kBwdMatBias;
   const int mode = bias_mode | (ext && prm.ex.dropout ? fo::kBwdDropout : 0);
 #define FO_BWD_MODE(M)                                                                                     \
   case M:                                                                                                  \
-    if (Dk == 128) rc = bf16 ? launch_bwd<128, true, M>(tq, tk, tv, tdo, tdq, prm, s) : launch_bwd<128, false, M>(tq, tk, tv, tdo, tdq, prm, s); \
-    else rc = bf16 ? launch_bwd<64, true, M>(tq, tk, tv, tdo, tdq, prm, s) : launch_bwd<64, false, M>(tq, tk, tv, tdo, tdq, prm, s);            \
+    if (Dk == 128) rc = bf16 ? fo::launch_bwd<128, true, M>(tq, tk, tv, tdo, tdq, prm, s) : fo::launch_bwd<128, false, M>(tq, tk, tv, tdo, tdq, prm, s); \
+    else rc = bf16 ? fo::launch_bwd<64, true, M>(tq, tk, tv, tdo, tdq, prm, s) : fo::launch_bwd<64, false, M>(tq, tk, tv, tdo, tdq, prm, s);            \
     break;
   // head_dim 72 to 96 without bias and dropout: matmuls of width 96 in the 128-column tiles
   // (B1 H48 Sq1000 Sk1531 D80 106 to 94 us, B1 H32 S4096 D96 causal 371 to 315); other sizes compute the
   // zero columns of the next tile width.
-  if (mode == 0 && D > 64 && D <= 96)
-    rc = bf16 ? launch_bwd<128, true, 0, 96>(tq, tk, tv, tdo, tdq, prm, s) : launch_bwd<128, false, 0, 96>(tq, tk, tv, tdo, tdq, prm, s);
+  if (rel)
+    rc = fo::launch_bwd_rel(tq, tk, tv, tdo, tdq, prm, bf16, s);
+  else if (mode == 0 && D > 64 && D <= 96)
+    rc = bf16 ? fo::launch_bwd<128, true, 0, 96>(tq, tk, tv, tdo, tdq, prm, s) : fo::launch_bwd<128, false, 0, 96>(tq, tk, tv, tdo, tdq, prm, s);
   else switch (mode) {
     FO_BWD_MODE(0)
     FO_BWD_MODE(1)
@@ -236,9 +223,9 @@ extern "C" int fo_flash_attn_bwd(const void* q, const void* k, const void* v, co
                                  const int64_t dv_strides[3],
                                  int dtype, int causal, float softmax_scale, int device, void* stream) {
   fo::clear_error();
-  return attn_bwd_impl(q, k, v, o, dout, lse, dq, dk, dv, dq_accum, delta, B, H, Sq, Sk, D, q_strides, k_strides,
-                       v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, dtype, causal,
-                       softmax_scale, nullptr, device, stream);
+  return fo::attn_bwd_impl(q, k, v, o, dout, lse, dq, dk, dv, dq_accum, delta, B, H, Sq, Sk, D, q_strides, k_strides,
+                           v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, dtype, causal,
+                           softmax_scale, nullptr, nullptr, device, stream);
 }
 
 extern "C" int fo_flash_attn_bwd_ex(const void* q, const void* k, const void* v, const void* o, const void* dout,
@@ -257,7 +244,7 @@ extern "C" int fo_flash_attn_bwd_ex(const void* q, const void* k, const void* v,
   fo::AttnExtras ex;
   if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset))
     return rc;
-  return attn_bwd_impl(q, k, v, o, dout, lse, dq, dk, dv, dq_accum, delta, B, H, Sq, Sk, D, q_strides, k_strides,
-                       v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, dtype, causal,
-                       softmax_scale, &ex, device, stream);
+  return fo::attn_bwd_impl(q, k, v, o, dout, lse, dq, dk, dv, dq_accum, delta, B, H, Sq, Sk, D, q_strides, k_strides,
+                           v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, dtype, causal,
+                           softmax_scale, &ex, nullptr, device, stream);
 }

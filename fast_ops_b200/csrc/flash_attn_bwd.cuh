@@ -63,6 +63,7 @@ struct AttnBwdParams {
   unsigned long long* trace;  // optional timeline of CTA (0,0) (debug), or null
   int device;  // device index of the launch (host side only)
   AttnExtras ex;  // bias / dropout of the forward; read only by the kernel variants built for them
+  RelBias rel;    // read only by the kernel variants built for a relative position bias
 };
 
 __device__ __forceinline__ void bwd_trace(const AttnBwdParams& prm, int role, int it, int ev) {
@@ -84,8 +85,9 @@ __device__ __forceinline__ void store_swizzled_unit(uint8_t* tile, int r, int u,
 
 
 // kExt, the variants compiled: bit 0 a bias that is the same for every query row ("vector"), bit 1
-// dropout, bit 2 a bias with a row stride ("matrix").
-constexpr int kBwdVecBias = 1, kBwdDropout = 2, kBwdMatBias = 4;
+// dropout, bit 2 a bias with a row stride ("matrix"), bit 3 a relative position bias with the gradient of
+// its table (a vector bias beside it is looked for at run time).
+constexpr int kBwdVecBias = 1, kBwdDropout = 2, kBwdMatBias = 4, kBwdRelBias = 8;
 
 template <int D, int kExt>
 struct BwdConfig {
@@ -178,6 +180,23 @@ __device__ __forceinline__ void load_bias_rows32(const AttnExtras& ex, const uin
   }
 }
 
+// Adds a warp's sums, one per lane, to the buckets of their relative positions `d`.  Lanes of one bucket
+// are neighbours (d ascends with the lane, or is the same in all): each run is summed into its first lane,
+// which adds it to the accumulator.  The accumulator belongs to this warp alone, so the order of the
+// additions does not change from run to run.
+__device__ __forceinline__ void add_diagonals(const RelBias& rel, float* acc, int d, int lane, float sum) {
+  const int bucket = __ldg(rel.bucket_of + d + rel.zero);
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const float v = __shfl_down_sync(0xffffffffu, sum, off);
+    const int other = __shfl_down_sync(0xffffffffu, bucket, off);
+    if (lane + off < 32 && other == bucket) sum += v;
+  }
+  const int before = __shfl_up_sync(0xffffffffu, bucket, 1);
+  if (lane == 0 || before != bucket) atomicAdd(acc + bucket, sum);
+  __syncwarp();
+}
+
 // grid = (key tiles, B*H); block = BwdConfig<D, kExt>::kThreads.
 // kMma is the head_dim that the matmuls compute, D the width of the tiles: the zero columns between
 // them are left out of the K Q^T and V dO^T steps and of the width of dV, dK and dQ.
@@ -234,7 +253,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const int n_q_tiles = (prm.Sq + kBlockM - 1) / kBlockM;
   // query tiles that see this key tile: all of them, or with a causal mask those whose last
   // row is not above the tile's first key
-  const int i0 = prm.causal ? min(j, n_q_tiles) : 0;
+  constexpr bool rel_bias = (kExt & kBwdRelBias) != 0;
+  const int q_off = rel_bias ? prm.rel.offset : 0;  // query row i stands at key position i + q_off
+  const int i0 = prm.causal ? min(rel_bias ? max(k0 - q_off, 0) / kBlockM : j, n_q_tiles) : 0;
   const int n_iter = n_q_tiles - i0;
   int* const dstat = prm.device_status;
 
@@ -321,12 +342,39 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                  (b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h + min(key, prm.Sk - 1)) * esize;
       if (vec_bias && key_ok) bias_key = load_bias1<kBf16>(prm.ex, bias_col, 0);
     }
+    // A relative bias: its values for this key by query row (read only near the diagonal), and the two far
+    // constants.
+    const float* rel_col = nullptr;
+    float rel_left = 0.f, rel_right = 0.f;
+    float* rel_acc = nullptr;
+    float2* rel_sums = nullptr;  // of query tile 0
+    const int64_t rel_sums_step = static_cast<int64_t>(gridDim.x) * kCW;
+    const int warp_key = k0 + (warp & 3) * 32 - q_off;  // query row that the warp's first key stands beside
+    if constexpr (rel_bias) {
+      rel_col = prm.rel.values + static_cast<int64_t>(h) * prm.rel.width;
+      rel_left = __ldg(rel_col);
+      rel_right = __ldg(rel_col + prm.rel.width - 1);
+      rel_col += static_cast<int64_t>(prm.rel.zero) + key - q_off;
+      if (prm.ex.bias != nullptr && key_ok)
+        bias_key = scaled_or_masked(load_elem<kBf16>(static_cast<const uint8_t*>(prm.ex.bias),
+                                                     b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h + key, prm.ex.bias_f32));
+      if (prm.rel.acc != nullptr) {
+        rel_acc = prm.rel.acc + ((static_cast<int64_t>(bh) * gridDim.x + j) * kCW + warp) * prm.rel.num_buckets;
+        for (int x = lane; x < prm.rel.num_buckets; x += 32) rel_acc[x] = 0.f;
+        __syncwarp();
+        rel_sums = prm.rel.tile_sums + (static_cast<int64_t>(bh) * n_q_tiles * gridDim.x + j) * kCW + warp;
+      }
+    }
     for (int it = 0; it < n_iter; ++it) {
       const int i = i0 + it;
       const int q0 = i * kBlockM;
       const int qc0 = q0 + part * kCols;  // first query of this thread's columns
       // masks are rare (diagonal tiles, a ragged last key tile); rows past Sq have -LSE = -inf
-      const bool need_mask = !key_ok || (prm.causal && k0 + kBlockN - 1 > q0);
+      const bool need_mask = !key_ok || (prm.causal && k0 + kBlockN - 1 > q0 + q_off);
+      // relative positions of the warp's 32 keys and its query columns: d_first to d_first + 30 + kCols
+      const int d_first = warp_key - (qc0 + kCols - 1);
+      const RelSide side = rel_bias ? rel_side(prm.rel, d_first, d_first + 30 + kCols) : kRelNear;
+      const bool rel_near = side == kRelNear;
       // What does not depend on S^T comes first: the keep decisions and the first bias values.
       uint32_t keep[kPieces];  // dropout: bit x of keep[cc] = element kept
       if constexpr (has_drop) {
@@ -349,7 +397,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         load_bias_rows32<kBf16>(prm.ex, bias_col + static_cast<int64_t>(q) * prm.ex.bias_stride_q * (prm.ex.bias_f32 ? 4 : 2),
                                 prm.Sq - q, bias_v);
       };
+      auto load_rel_piece = [&](int cc) {  // near the diagonal: this key's bias for 32 consecutive query rows
+        const float* const p = rel_col - (qc0 + cc * 32);
+#pragma unroll
+        for (int x = 0; x < 32; ++x) bias_v[x] = __ldg(p - x) + bias_key;
+      };
       if constexpr (mat_bias) load_bias_piece(0);
+      if constexpr (rel_bias) {
+        if (rel_near) load_rel_piece(0);
+      }
+      const float rel_far = bias_key + (side == kRelLeft ? rel_left : rel_right);
       mbar_wait(bar_lse_full + Cfg::par(it), Cfg::phase(it), cta_abort, dstat, FO_STATUS_TIMEOUT_TMA);
       mbar_wait(bar_s_full, it & 1, cta_abort, dstat, FO_STATUS_TIMEOUT_MMA);
       tcgen05_fence_after_sync();
@@ -365,6 +422,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if constexpr (mat_bias) {
           if (cc > 0) load_bias_piece(cc);
         }
+        if constexpr (rel_bias) {
+          if (rel_near && cc > 0) load_rel_piece(cc);
+          if (!rel_near) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) bias_v[x] = rel_far;
+          }
+        }
 #pragma unroll
         for (int x = 0; x < 32; x += 4) {
           const float4 t = *reinterpret_cast<const float4*>(nl + x);  // broadcast read
@@ -373,7 +437,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           for (int y = 0; y < 4; ++y) {
             const float sv = __uint_as_float(sr[cc][x + y]);
             float e;
-            if constexpr (mat_bias) e = fmaf(sv, prm.scale_log2, bias_v[x + y]) + nlv[y];
+            if constexpr (mat_bias || rel_bias) e = fmaf(sv, prm.scale_log2, bias_v[x + y]) + nlv[y];
             else if constexpr (vec_bias) e = fmaf(sv, prm.scale_log2, bias_key) + nlv[y];
             else e = fmaf(sv, prm.scale_log2, nlv[y]);
             sr[cc][x + y] = __float_as_uint(fast_exp2(e));
@@ -383,7 +447,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
           for (int x = 0; x < 32; ++x) {
             const int q = qc0 + cc * 32 + x;
-            if (!key_ok || (prm.causal && key > q)) sr[cc][x] = 0u;
+            if (!key_ok || (prm.causal && key > q + q_off)) sr[cc][x] = 0u;
           }
         }
       }
@@ -418,6 +482,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // query tile's dP^T matmul.
         uint8_t* const ds_tile = sDS + (it & (Cfg::kSlots - 1)) * Cfg::kDSBytes;
         uint32_t dd[kPieces * 16];
+        // Table gradient: the sum of dS over the part, and near the diagonal also along the diagonals of its
+        // 32-column pieces: the value of key row r and column x goes to lane (r - x) mod 32, where those
+        // with r >= x and those with r < x are two diagonals 32 apart.  diag[k]: relative position
+        // d_first + kCols - 1 + lane - 32 k.
+        const bool diag_sums = rel_bias && rel_near && rel_acc != nullptr;
+        float diag[kPieces + 1];
+        float2 far_sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k <= kPieces; ++k) diag[k] = 0.f;
 #pragma unroll
         for (int cc = 0; cc < kPieces; ++cc) {
           const float* nd = sNegDelta + (it & (Cfg::kSlots - 1)) * 128 + part * kCols + cc * 32;
@@ -437,6 +510,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               }
               dsv[y] = __uint_as_float(sr[cc][x + y]) * fmaf(g, dp_scale, ndv[y]);
             }
+            if constexpr (rel_bias) {
+              if (diag_sums) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                  const float v = __shfl_sync(0xffffffffu, dsv[y], (lane + x + y) & 31);
+                  if (lane + x + y < 32) diag[cc] += v;
+                  else diag[cc + 1] += v;
+                }
+              } else {
+                far_sum = __fadd2_rn(far_sum, __fadd2_rn(make_float2(dsv[0], dsv[1]), make_float2(dsv[2], dsv[3])));
+              }
+            }
             dd[cc * 16 + (x >> 1)] = pack2<kBf16>(dsv[0], dsv[1]);
             dd[cc * 16 + (x >> 1) + 1] = pack2<kBf16>(dsv[2], dsv[3]);
           }
@@ -445,12 +530,37 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
         for (int u = 0; u < kPieces * 4; ++u)
           store_swizzled_unit(ds_tile, r, part * kPieces * 4 + u, make_uint4(dd[4 * u], dd[4 * u + 1], dd[4 * u + 2], dd[4 * u + 3]));
+        tcgen05_wait_st();
+        fence_proxy_async_smem();  // shared-memory writes of these threads must be visible to the tensor core's reads
+        tcgen05_fence_before_sync();
+        mbar_arrive(bar_ds_full + Cfg::par(it));
+        if (warp == 0) bwd_trace(prm, 0, it, 1);
+        if constexpr (rel_bias) {
+          if (rel_acc != nullptr) {
+            float ds_sum = far_sum.x + far_sum.y, p_sum = 0.f;
+            if (diag_sums) {
+#pragma unroll
+              for (int k = 0; k <= kPieces; ++k) {
+                ds_sum += diag[k];
+                add_diagonals(prm.rel, rel_acc, d_first + kCols - 1 + lane - 32 * k, lane, diag[k]);
+              }
+            }
+            float2 p2 = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int cc = 0; cc < kPieces; ++cc)
+#pragma unroll
+              for (int x = 0; x < 32; x += 2)
+                p2 = __fadd2_rn(p2, make_float2(__uint_as_float(sr[cc][x]), __uint_as_float(sr[cc][x + 1])));
+            p_sum = p2.x + p2.y;
+#pragma unroll
+            for (int off = 16; off >= 1; off >>= 1) {
+              ds_sum += __shfl_xor_sync(0xffffffffu, ds_sum, off);
+              p_sum += __shfl_xor_sync(0xffffffffu, p_sum, off);
+            }
+            if (lane == 0) rel_sums[i * rel_sums_step] = make_float2(ds_sum, p_sum);
+          }
+        }
       }
-      tcgen05_wait_st();
-      fence_proxy_async_smem();  // shared-memory writes of these threads must be visible to the tensor core's reads
-      tcgen05_fence_before_sync();
-      mbar_arrive(bar_ds_full + Cfg::par(it));
-      if (warp == 0) bwd_trace(prm, 0, it, 1);
     }
 
     // ---- epilogue: key row (k0 + r); the first half of the warps write dK, the second dV ----
@@ -724,6 +834,19 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   tcgen05_fence_before_sync();
   __syncthreads();
   if (warp == kCW + 4) tmem_dealloc(tmem_base, Cfg::kTmemCols);
+}
+
+template <int D, bool kBf16, int kExt, int kMma = D>
+int launch_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
+               const CUtensorMap& tdq, const AttnBwdParams& prm, cudaStream_t stream) {
+  dim3 grid((prm.Sk + kBlockN - 1) / kBlockN, prm.B * prm.H);
+  auto kernel = attn_bwd_kernel<D, kBf16, kExt, kMma>;
+  constexpr int smem = BwdConfig<D, kExt>::kSmemBytes;
+  FO_CUDA_CHECK((ensure_dynamic_smem<attn_bwd_kernel<D, kBf16, kExt, kMma>>(smem, prm.device)));
+  kernel<<<grid, BwdConfig<D, kExt>::kThreads, smem, stream>>>(tq, tk, tv, tdo, tdq, prm);
+  g_launch_count.fetch_add(1, std::memory_order_relaxed);
+  FO_CUDA_CHECK(cudaGetLastError());
+  return FO_OK;
 }
 
 }  // namespace fo

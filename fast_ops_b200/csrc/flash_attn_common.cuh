@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 
 #include "fo_ptx.cuh"
+#include "rel_bias.cuh"
 
 namespace fo {
 
@@ -88,8 +89,9 @@ __device__ __forceinline__ void load_bias32(const AttnExtras& ex, const uint8_t*
 }
 
 // kExt of the 64-key kernel for a bias, the variants compiled: a bias that is the same for every query row
-// ("vector"), dropout, a 16-bit or an fp32 bias with a row stride ("matrix").
-constexpr int kFwdVecBias = 1, kFwdDropout = 2, kFwdMatBias = 4, kFwdMatBias32 = 8;
+// ("vector"), dropout, a 16-bit or an fp32 bias with a row stride ("matrix"), a bias of the relative
+// position (alone, or with a vector bias).
+constexpr int kFwdVecBias = 1, kFwdDropout = 2, kFwdMatBias = 4, kFwdMatBias32 = 8, kFwdRelBias = 16;
 
 struct AttnParams {
   void* o;
@@ -115,6 +117,7 @@ struct AttnParams {
   // Persistent kernels: two words in global memory, zero at launch, that the launch's CTAs use to
   // hand out work items ([0]) and to find the last CTA, which zeroes them again ([1]).
   int* sched;
+  RelBias rel;  // read only by the kernels built for a relative position bias
 };
 
 // One element of a bias row as log2(e) * value; `base` points at column 0 of the row.
@@ -125,6 +128,15 @@ __device__ __forceinline__ float load_bias1(const AttnExtras& ex, const uint8_t*
   const uint16_t h = __ldg(reinterpret_cast<const uint16_t*>(base) + col);
   if constexpr (kBf16) return __uint_as_float(static_cast<uint32_t>(h) << 16) * kLog2e;
   else return __half2float(__ushort_as_half(h)) * kLog2e;
+}
+
+// Element `i` of an fp32 or 16-bit array.
+template <bool kBf16>
+__device__ __forceinline__ float load_elem(const uint8_t* base, int64_t i, int f32) {
+  if (f32) return __ldg(reinterpret_cast<const float*>(base) + i);
+  const uint16_t h = __ldg(reinterpret_cast<const uint16_t*>(base) + i);
+  if constexpr (kBf16) return __uint_as_float(static_cast<uint32_t>(h) << 16);
+  else return __half2float(__ushort_as_half(h));
 }
 
 // L2 prefetch of the `ncols` bias elements of a row starting at column col0 (row pointer non-null,

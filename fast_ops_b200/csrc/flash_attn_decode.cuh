@@ -1,5 +1,6 @@
 // Attention forward for a single query row per head (decoding one token against stored keys and
-// values): softmax(scale q K^T) V with Sq = 1, no mask, bias or dropout.
+// values): softmax(scale q K^T) V with Sq = 1, no dropout; no bias either, or a relative position bias with
+// or without a vector bias.
 //
 // Bound by memory: every key and value is used by one query row (or, when the heads share one K/V
 // head, by one row of each), so the 128-row tensor-core tiles of the other kernels would do 1/128
@@ -23,6 +24,7 @@
 #include <cooperative_groups.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "flash_attn_common.cuh"
 #include "fo_host.h"
@@ -43,6 +45,20 @@ struct DecodeParams {
   const int* device_status;
 };
 
+// No bias, or (DecodeRel) what the kernel needs to find the bias of a key's relative position by itself: with one
+// query row a bias vector expanded beforehand would be read once, and its launch would cost more.
+struct NoRel {};
+struct DecodeRel {
+  RelBuckets buckets;
+  const uint8_t* table;  // values of the whole table, fp32 or the 16-bit type of Q
+  int64_t stride_bucket, stride_head;
+  int table_f32;
+  int offset;            // key position of the query
+  const uint8_t* bias;   // vector bias beside it (element (b, h, j) at bias + b*s_b + h*s_h + j), or null
+  int64_t bias_stride_b, bias_stride_h;
+  int bias_f32;
+};
+
 __device__ __forceinline__ uint4 ldg_stream(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -55,9 +71,10 @@ __device__ __forceinline__ uint4 ldg_stream(const void* p) {
 template <int kHeads, int kWarps>
 constexpr int kDecodePerSm = (kHeads == 1 ? 16 : 8) / kWarps;
 
-template <int D, bool kBf16, int kHeads, int kWarps>
+template <int D, bool kBf16, int kHeads, int kWarps, class Rel = NoRel>
 __global__ void __launch_bounds__(kWarps * 32, kDecodePerSm<kHeads, kWarps>)
-attn_decode_kernel(const DecodeParams prm) {
+attn_decode_kernel(const DecodeParams prm, const __grid_constant__ Rel rel) {
+  constexpr bool kRel = !std::is_same<Rel, NoRel>::value;
   namespace cg = cooperative_groups;
   constexpr int kLanes = D / 8;        // lanes per key row
   constexpr int kGroups = 32 / kLanes; // rows a warp loads per instruction
@@ -122,11 +139,35 @@ attn_decode_kernel(const DecodeParams prm) {
   const int own = (kLanes == 8) ? sub : (sub >> 1);
   const bool counts = (kLanes == 8) || (sub & 1) == 0;  // one lane per row adds it to the sum
 
+  // Most keys are farther from the query than the last bucket's start: one value per head.
+  float rel_far[kHeads];
+  if constexpr (kRel) {
+#pragma unroll
+    for (int r = 0; r < kHeads; ++r)
+      rel_far[r] = scaled_or_masked(load_elem<kBf16>(
+          rel.table, (rel.buckets.n - 1) * rel.stride_bucket + min(h0 + r, prm.H - 1) * rel.stride_head, rel.table_f32));
+  }
+
   uint4 kw[kBatch], vw[kBatch];
   int base = begin + warp * kStep;
   if (base < end) load_rows(kw, kp, prm.k_stride_s, base);
   for (; base < end; base += kWarps * kStep) {
     load_rows(vw, vp, prm.v_stride_s, base);
+    float bias[kHeads];  // of this lane's key, times log2(e)
+    if constexpr (kRel) {
+      const int key = min(base + group * kBatch + own, prm.Sk - 1);
+      const int d = key - rel.offset;
+      const bool far = d <= -rel.buckets.starts[rel.buckets.n - 1];
+      const int bucket = far ? 0 : rel_bucket(rel.buckets, d);
+#pragma unroll
+      for (int r = 0; r < kHeads; ++r) {
+        const int h = min(h0 + r, prm.H - 1);
+        bias[r] = rel_far[r];
+        if (!far) bias[r] = scaled_or_masked(load_elem<kBf16>(rel.table, bucket * rel.stride_bucket + h * rel.stride_head, rel.table_f32));
+        if (rel.bias != nullptr)
+          bias[r] += scaled_or_masked(load_elem<kBf16>(rel.bias, b * rel.bias_stride_b + h * rel.bias_stride_h + key, rel.bias_f32));
+      }
+    }
     float s[kHeads];
 #pragma unroll
     for (int r = 0; r < kHeads; ++r) {
@@ -152,6 +193,7 @@ attn_decode_kernel(const DecodeParams prm) {
         }
       }
       if constexpr (kLanes > kScatter) t[0] += __shfl_xor_sync(0xffffffffu, t[0], 1);
+      if constexpr (kRel) t[0] += bias[r];
       s[r] = (base + group * kBatch + own < end) ? t[0] : -INFINITY;
     }
     // K of the next step: its registers are free now
@@ -328,9 +370,9 @@ inline DecodeShape decode_shape(int B, int H, int Sk, int D, bool shared_kv, int
 // CTAs), while a CTA keeps at least 128 keys.  Measured at splits 1 / 2 / 4 / 8 / 16 (us):
 // B4 H32 Sk4096 D128 57 / 43 / 46 / 52 / 79 (takes 2); B1 H8 Sk32768 D128 389 / 197 / 101 / 54 / 36
 // (16); B8 H40 Sk3000 D96 92 / 82 / 80 / 96 (4).
-template <int D, bool kBf16, int kHeads, int kWarps>
-int launch_decode(const DecodeParams& base, int B, int split, int num_sms, int device, cudaStream_t stream) {
-  constexpr auto kernel = attn_decode_kernel<D, kBf16, kHeads, kWarps>;
+template <int D, bool kBf16, int kHeads, int kWarps, class Rel = NoRel>
+int launch_decode(const DecodeParams& base, const Rel& rel, int B, int split, int num_sms, int device, cudaStream_t stream) {
+  constexpr auto kernel = attn_decode_kernel<D, kBf16, kHeads, kWarps, Rel>;
   const int64_t groups = static_cast<int64_t>((base.H + kHeads - 1) / kHeads) * B;
   if (split == 0) {
     const int resident = num_sms * kDecodePerSm<kHeads, kWarps>;
@@ -358,7 +400,7 @@ int launch_decode(const DecodeParams& base, int B, int split, int num_sms, int d
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  FO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, prm));
+  FO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, prm, rel));
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   return FO_OK;
 }

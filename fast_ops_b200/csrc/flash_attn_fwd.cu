@@ -11,6 +11,7 @@
 #include <mutex>
 
 #include "flash_attn_decode.cuh"
+#include "flash_attn_host.h"
 #include "flash_attn_simple.cuh"
 #include "flash_attn_ws.cuh"
 #include "flash_attn_ws64.cuh"
@@ -220,7 +221,8 @@ int make_attn_extras(AttnExtras* ex, const void* bias, const int64_t* bias_strid
 // Launches the split-key kernel; strides are those check_layout returned, in elements.
 static int decode(const void* q, const void* k, const void* v, void* o, float* lse, int B, int H, int Sk, int D,
                   const int64_t qs[3], const int64_t ks[3], const int64_t vs[3], const int64_t os[3], bool kv_bcast,
-                  int dtype, float softmax_scale, const int* status, int num_sms, int device, cudaStream_t stream) {
+                  int dtype, float softmax_scale, const int* status, const fo::RelArgs* rel, const fo::AttnExtras* ex,
+                  int num_sms, int device, cudaStream_t stream) {
   fo::DecodeParams prm;
   prm.q = static_cast<const uint16_t*>(q);
   prm.k = static_cast<const uint16_t*>(k);
@@ -243,12 +245,13 @@ static int decode(const void* q, const void* k, const void* v, void* o, float* l
   prm.scale_log2 = softmax_scale * 1.4426950408889634f;
   prm.device_status = status;
   const bool bf16 = dtype == FO_BF16;
+  if (rel) return fo::launch_decode_rel(prm, *rel, *ex, B, H, Sk, D, kv_bcast, bf16, num_sms, device, stream);
   // Heads that share K and V may go four to a CTA, so that the shared tensors cross L2 a quarter as often.
   const fo::DecodeShape shape = fo::decode_shape(B, H, Sk, D, kv_bcast, num_sms);
 #define FO_DECODE(DK, HEADS, WARPS)                                                                                \
   if ((DK == 64) == (D <= 64) && shape.heads == HEADS && shape.warps == WARPS)                                     \
-    return bf16 ? fo::launch_decode<DK, true, HEADS, WARPS>(prm, B, shape.split, num_sms, device, stream)          \
-                : fo::launch_decode<DK, false, HEADS, WARPS>(prm, B, shape.split, num_sms, device, stream);
+    return bf16 ? fo::launch_decode<DK, true, HEADS, WARPS>(prm, {}, B, shape.split, num_sms, device, stream)      \
+                : fo::launch_decode<DK, false, HEADS, WARPS>(prm, {}, B, shape.split, num_sms, device, stream);
 #define FO_DECODE_WARPS(DK, HEADS) FO_DECODE(DK, HEADS, 8) FO_DECODE(DK, HEADS, 4) FO_DECODE(DK, HEADS, 2)
   FO_DECODE_WARPS(64, 1)
   FO_DECODE_WARPS(64, 4)
@@ -259,12 +262,12 @@ static int decode(const void* q, const void* k, const void* v, void* o, float* l
   return fo::fail(FO_ERR_UNSUPPORTED, "no decoding kernel of this shape");
 }
 
-static int attn_fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse,
-                         int B, int H, int Sq, int Sk, int D,
-                         const int64_t q_strides[3], const int64_t k_strides[3],
-                         const int64_t v_strides[3], const int64_t o_strides[3],
-                         int dtype, int causal, float softmax_scale, const fo::AttnExtras* ex,
-                         int device, void* stream) {
+int fo::attn_fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse,
+                      int B, int H, int Sq, int Sk, int D,
+                      const int64_t q_strides[3], const int64_t k_strides[3],
+                      const int64_t v_strides[3], const int64_t o_strides[3],
+                      int dtype, int causal, float softmax_scale, const fo::AttnExtras* ex, const fo::RelArgs* rel,
+                      int device, void* stream) {
   FO_REQUIRE(q && k && v && o, "null tensor pointer");
   FO_REQUIRE(q_strides && k_strides && v_strides && o_strides, "null stride array");
   FO_REQUIRE(dtype == FO_F16 || dtype == FO_BF16, "attention inputs must be fp16 or bf16 (got dtype %d)", dtype);
@@ -293,15 +296,20 @@ static int attn_fwd_impl(const void* q, const void* k, const void* v, void* o, f
   const DeviceInfo* info = device_info(device);
   if (!info) return fo::fail(FO_ERR_CUDA, "cannot look up device %d", device);
   AttnImpl impl = static_cast<AttnImpl>(fo::g_attn_options.impl.load(std::memory_order_relaxed));
-  if (impl == AttnImpl::kAuto && Sq == 1 && !causal && !ext) {
-    // One query row per head: the split-key kernel.  (With a causal mask only key 0 is visible.)
+  // One query row per head: the split-key kernel.  (With a causal mask only key 0 is visible, or with a
+  // relative bias those up to the query's own position.)
+  const bool rel_decode = rel && Sq == 1 && !ex->dropout;
+  const int keys = rel && causal ? std::min(Sk, rel->bias.offset + 1) : Sk;
+  if (rel_decode || (!rel && impl == AttnImpl::kAuto && Sq == 1 && !causal && !ext)) {
     int64_t qs[3], ks[3], vs[3];
     if (int rc = fo::check_layout(q, B, H, Sq, D, q_strides, "q", qs)) return rc;
     FO_REQUIRE(kv_same, "k and v must both have a head stride, or both be expanded with head stride 0");
     if (int rc = fo::check_layout(k, B, Hkv, Sk, D, k_strides, "k", ks)) return rc;
     if (int rc = fo::check_layout(v, B, Hkv, Sk, D, v_strides, "v", vs)) return rc;
-    return decode(q, k, v, o, lse, B, H, Sk, D, qs, ks, vs, o_strides, kv_bcast, dtype, softmax_scale, status, info->num_sms,
-                  device, static_cast<cudaStream_t>(stream));
+    if (rel && lse != nullptr)  // a backward may follow, whose tile kernels read the expanded bias
+      if (int rc = fo::launch_rel_expand(*rel, H, dtype == FO_BF16, static_cast<cudaStream_t>(stream))) return rc;
+    return decode(q, k, v, o, lse, B, H, rel ? keys : Sk, D, qs, ks, vs, o_strides, kv_bcast, dtype, softmax_scale, status,
+                  rel, ex, info->num_sms, device, static_cast<cudaStream_t>(stream));
   }
 
   CUtensorMap tq, tk, tv;
@@ -334,6 +342,8 @@ static int attn_fwd_impl(const void* q, const void* k, const void* v, void* o, f
   std::memset(&prm.ex, 0, sizeof(prm.ex));
   prm.ex.drop_rescale = 1.f;
   if (ext) prm.ex = *ex;
+  std::memset(&prm.rel, 0, sizeof(prm.rel));
+  if (rel) prm.rel = rel->bias;
   {
     // as many heads per group as keep their K and V (2 * Sk * D * 2 bytes each) within about a
     // third of the 126 MB L2, leaving room for Q, O and the other traffic
@@ -348,6 +358,10 @@ static int attn_fwd_impl(const void* q, const void* k, const void* v, void* o, f
 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == FO_BF16;
+  if (rel) {
+    if (int rc = fo::launch_rel_expand(*rel, H, bf16, s)) return rc;
+    return fo::launch_fwd_rel(tq, tk, tv, prm, bf16, s);
+  }
   if (impl == AttnImpl::kAuto) {
     // The 64-key-step kernel is the faster one at every shape measured (same box, hot loop, bf16
     // causal: S=16384 1.11 against 1.02 PFLOP/s, S=4096 0.98 against 0.82, GPT-2-small shape
@@ -425,8 +439,8 @@ extern "C" int fo_flash_attn_fwd(const void* q, const void* k, const void* v, vo
                                  const int64_t v_strides[3], const int64_t o_strides[3],
                                  int dtype, int causal, float softmax_scale, int device, void* stream) {
   fo::clear_error();
-  return attn_fwd_impl(q, k, v, o, lse, B, H, Sq, Sk, D, q_strides, k_strides, v_strides, o_strides, dtype, causal,
-                       softmax_scale, nullptr, device, stream);
+  return fo::attn_fwd_impl(q, k, v, o, lse, B, H, Sq, Sk, D, q_strides, k_strides, v_strides, o_strides, dtype, causal,
+                           softmax_scale, nullptr, nullptr, device, stream);
 }
 
 extern "C" int fo_flash_attn_fwd_ex(const void* q, const void* k, const void* v, void* o, float* lse,
@@ -442,8 +456,8 @@ extern "C" int fo_flash_attn_fwd_ex(const void* q, const void* k, const void* v,
   fo::AttnExtras ex;
   if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset))
     return rc;
-  return attn_fwd_impl(q, k, v, o, lse, B, H, Sq, Sk, D, q_strides, k_strides, v_strides, o_strides, dtype, causal,
-                       softmax_scale, &ex, device, stream);
+  return fo::attn_fwd_impl(q, k, v, o, lse, B, H, Sq, Sk, D, q_strides, k_strides, v_strides, o_strides, dtype, causal,
+                           softmax_scale, &ex, nullptr, device, stream);
 }
 
 // out[b, h, i, j] = 1 if element (i, j) of head (b, h) is kept by the dropout of

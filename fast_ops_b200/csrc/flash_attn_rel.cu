@@ -1,0 +1,369 @@
+// Attention with a learned relative position bias (rel_bias.cuh): entry points, the launches of the tile
+// and decoding kernels built for it, and the two small kernels around them: the bias of a head as a vector
+// over the relative position, and the gradient of the table from the backward's partial sums.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "flash_attn_bwd.cuh"
+#include "flash_attn_decode.cuh"
+#include "flash_attn_host.h"
+#include "flash_attn_ws64r.cuh"
+#include "fo_host.h"
+
+namespace {
+
+using fo::RelArgs;
+using fo::RelBias;
+using fo::RelBuckets;
+
+// values[h][x] = log2(e) * table[bucket(x - zero)][h], and the buckets themselves.
+template <bool kBf16>
+__global__ void __launch_bounds__(256)
+rel_expand_kernel(const __grid_constant__ RelBuckets buckets, const uint8_t* __restrict__ table, int64_t stride_bucket,
+                  int64_t stride_head, int table_f32, int zero, int width, float* __restrict__ values,
+                  int* __restrict__ bucket_of) {
+  const int x = blockIdx.x * 256 + threadIdx.x;
+  const int h = blockIdx.y;
+  if (x >= width) return;
+  const int bucket = fo::rel_bucket(buckets, x - zero);
+  values[static_cast<int64_t>(h) * width + x] =
+      fo::scaled_or_masked(fo::load_elem<kBf16>(table, bucket * stride_bucket + h * stride_head, table_f32));
+  if (h == 0) bucket_of[x] = bucket;
+}
+
+template <class T>
+__device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// The table's gradient from the backward's partial sums (which carry the softmax scale, as dS of the other
+// gradients does): dtable[u][h] = 1 / scale * (sums of the parts that are far from the diagonal on the side
+// of u's bucket + sums by bucket of the parts near it).
+//
+// dS = P o (dP - delta) sums to zero over the keys of a query.  delta comes from an O whose P and whose
+// result were rounded to 16 bits; an error of it leaves P times that error in every dS of the row, with one
+// sign, which the far buckets collect over thousands of keys: 0.5 to 1 % of their gradient at S = 4096 to 8192.
+// What the sums over all keys of a block of queries miss zero by is that error's sum over the block; it
+// is put back in proportion to the probability mass that each side holds of the block's queries.
+// One block per head: a warp per (batch, block of kCols queries) for the far sums, then all threads
+// for the sums by bucket, everything in a fixed order and in double.
+template <class T>
+__global__ void __launch_bounds__(1024)
+rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, int n_q_tiles, int n_k_tiles, int warps,
+                      int causal, float inv_scale) {
+  __shared__ double far[32][2];
+  __shared__ double part[32][33];
+  const int h = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int parts = warps / 4, cols = fo::kBlockM / parts;  // four warps share a part's queries
+  double left = 0, right = 0;
+  for (int64_t item = warp; item < static_cast<int64_t>(B) * n_q_tiles * parts; item += 32) {
+    const int p = static_cast<int>(item % parts);
+    const int64_t bi = item / parts;
+    const int i = static_cast<int>(bi % n_q_tiles);
+    const int64_t bh = bi / n_q_tiles * H + h;
+    const float2* const row = rel.tile_sums + (bh * n_q_tiles + i) * n_k_tiles * warps + p * 4;
+    const int q_first = i * fo::kBlockM + p * cols + rel.offset;  // key position of the part's first query
+    // key tiles that this query tile sees (the backward visits no others)
+    int n = n_k_tiles;
+    if (causal) n = min(n, (i * fo::kBlockM + fo::kBlockM - 1 + rel.offset) / fo::kBlockN + 1);
+    double ds = 0, mass = 0, ds_side[2] = {0, 0}, mass_side[2] = {0, 0};
+    for (int x = lane; x < n * 4; x += 32) {
+      const int key = x * 32;  // key tile x / 4, its quarter x % 4
+      const float2 v = row[static_cast<int64_t>(x >> 2) * warps + (x & 3)];
+      const int d_first = key - (q_first + cols - 1);
+      const fo::RelSide side = fo::rel_side(rel, d_first, d_first + 30 + cols);
+      ds += v.x;
+      mass += v.y;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        if (side == (w == 0 ? fo::kRelLeft : fo::kRelRight)) {
+          ds_side[w] += v.x;
+          mass_side[w] += v.y;
+        }
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) {
+      ds += __shfl_xor_sync(0xffffffffu, ds, off);
+      mass += __shfl_xor_sync(0xffffffffu, mass, off);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        ds_side[w] += __shfl_xor_sync(0xffffffffu, ds_side[w], off);
+        mass_side[w] += __shfl_xor_sync(0xffffffffu, mass_side[w], off);
+      }
+    }
+    if (mass > 0) {
+      left += ds_side[0] - ds * (mass_side[0] / mass);
+      right += ds_side[1] - ds * (mass_side[1] / mass);
+    }
+  }
+  if (lane == 0) {
+    far[warp][0] = left;
+    far[warp][1] = right;
+  }
+  __syncthreads();
+  const int left_bucket = rel.bucket_of[0], right_bucket = rel.bucket_of[rel.width - 1];
+  for (int u0 = 0; u0 < rel.num_buckets; u0 += 32) {
+    const int u = u0 + lane;
+    double sum = 0;
+    if (u < rel.num_buckets)
+      for (int b = 0; b < B; ++b) {
+        const float* const p = rel.acc + (static_cast<int64_t>(b) * H + h) * n_k_tiles * warps * rel.num_buckets + u;
+#pragma unroll 4
+        for (int i = warp; i < n_k_tiles * warps; i += 32) sum += static_cast<double>(p[static_cast<int64_t>(i) * rel.num_buckets]);
+      }
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && u < rel.num_buckets) {
+      for (int i = 1; i < 32; ++i) sum += part[i][lane];
+      for (int i = 0; i < 32; ++i) {
+        if (u == left_bucket) sum += far[i][0];
+        if (u == right_bucket) sum += far[i][1];
+      }
+      dtable[static_cast<int64_t>(u) * H + h] = from_f32<T>(static_cast<float>(sum * inv_scale));
+    }
+    __syncthreads();
+  }
+}
+
+// Checks of the relative bias's own arguments; fills everything of `rel` but the device pointers of the
+// expanded vector.
+int make_rel_args(RelArgs* rel, int Sq, int Sk, const void* table, int table_dtype, const int64_t* table_strides,
+                  const int* starts, int n_starts, int two_sided, int query_offset, int dtype) {
+  FO_REQUIRE(dtype == FO_F16 || dtype == FO_BF16, "attention inputs must be fp16 or bf16 (got dtype %d)", dtype);
+  FO_REQUIRE(table && table_strides && starts, "null relative bias argument");
+  FO_REQUIRE(table_dtype == FO_F32 || table_dtype == dtype, "the table must be fp32 or have the dtype of q (got dtype %d)",
+             table_dtype);
+  FO_REQUIRE(reinterpret_cast<uintptr_t>(table) % (table_dtype == FO_F32 ? 4 : 2) == 0, "the table is not aligned to its elements");
+  FO_REQUIRE(table_strides[0] >= 0 && table_strides[1] >= 0, "the table's strides must be non-negative");
+  FO_REQUIRE(n_starts >= 1 && n_starts <= fo::kRelMaxStarts, "1 to %d buckets per side (got %d)", fo::kRelMaxStarts, n_starts);
+  FO_REQUIRE(starts[0] == 0, "the first bucket must start at distance 0");
+  for (int i = 1; i < n_starts; ++i) FO_REQUIRE(starts[i] >= starts[i - 1], "bucket starts must not descend");
+  FO_REQUIRE(query_offset >= 0 && query_offset <= (1 << 29), "query_offset must be in [0, 2^29] (got %d)", query_offset);
+  FO_REQUIRE(Sq > 0 && Sk > 0 && Sq <= (1 << 29) && Sk <= (1 << 29), "Sq and Sk must be in [1, 2^29]");
+  std::memset(rel, 0, sizeof(*rel));
+  std::copy(starts, starts + n_starts, rel->buckets.starts);
+  rel->buckets.n = n_starts;
+  rel->buckets.two_sided = two_sided ? 1 : 0;
+  rel->table = table;
+  rel->stride_bucket = table_strides[0];
+  rel->stride_head = table_strides[1];
+  rel->table_f32 = table_dtype == FO_F32;
+  RelBias& bias = rel->bias;
+  bias.offset = query_offset;
+  bias.num_buckets = n_starts * (two_sided ? 2 : 1);
+  // no relative position of the call lies beyond these
+  const int last = starts[n_starts - 1];
+  bias.far_left = std::min(last, Sq + query_offset);
+  bias.far_right = two_sided ? std::min(std::max(last, 1), Sk) : 0;
+  bias.zero = bias.far_left + fo::kRelMargin;
+  bias.width = bias.zero + bias.far_right + fo::kRelMargin + 1;
+  return FO_OK;
+}
+
+int64_t expanded_bytes(const RelBias& bias, int H) { return (static_cast<int64_t>(H) + 1) * bias.width * 4; }
+
+void set_expanded(RelBias* bias, void* workspace, int H) {
+  bias->values = static_cast<const float*>(workspace);
+  bias->bucket_of = reinterpret_cast<const int*>(bias->values + static_cast<int64_t>(H) * bias->width);
+}
+
+// Warps of the backward that sum for the table's gradient, per key tile.
+int bwd_warps(int D, bool dropout) {
+  if (D > 64) return dropout ? fo::BwdConfig<128, fo::kBwdRelBias | fo::kBwdDropout>::kComputeWarps
+                             : fo::BwdConfig<128, fo::kBwdRelBias>::kComputeWarps;
+  return dropout ? fo::BwdConfig<64, fo::kBwdRelBias | fo::kBwdDropout>::kComputeWarps
+                 : fo::BwdConfig<64, fo::kBwdRelBias>::kComputeWarps;
+}
+
+// Floats of the backward's partial sums: float2 per tile and warp first, then the sums by bucket.
+int64_t tile_sum_floats(int B, int H, int Sq, int Sk, int D, bool dropout) {
+  return 2LL * B * H * ((Sq + fo::kBlockM - 1) / fo::kBlockM) * ((Sk + fo::kBlockN - 1) / fo::kBlockN) * bwd_warps(D, dropout);
+}
+
+int64_t bucket_sum_floats(int B, int H, int Sk, int D, int num_buckets, bool dropout) {
+  return 1LL * B * H * ((Sk + fo::kBlockN - 1) / fo::kBlockN) * bwd_warps(D, dropout) * num_buckets;
+}
+
+int check_bias_strides(const void* bias, const int64_t* strides) {
+  if (bias == nullptr) return FO_OK;
+  FO_REQUIRE(strides != nullptr, "bias given without strides");
+  FO_REQUIRE(strides[2] == 0, "beside a relative bias, bias must be the same for every query row (row stride 0)");
+  return FO_OK;
+}
+
+}  // namespace
+
+namespace fo {
+
+int launch_rel_expand(const RelArgs& rel, int H, bool bf16, cudaStream_t stream) {
+  const dim3 grid((rel.bias.width + 255) / 256, H);
+  auto kernel = bf16 ? rel_expand_kernel<true> : rel_expand_kernel<false>;
+  kernel<<<grid, 256, 0, stream>>>(rel.buckets, static_cast<const uint8_t*>(rel.table), rel.stride_bucket, rel.stride_head,
+                                   rel.table_f32, rel.bias.zero, rel.bias.width, const_cast<float*>(rel.bias.values),
+                                   const_cast<int*>(rel.bias.bucket_of));
+  g_launch_count.fetch_add(1, std::memory_order_relaxed);
+  FO_CUDA_CHECK(cudaGetLastError());
+  return FO_OK;
+}
+
+int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& prm, bool bf16,
+                   cudaStream_t stream) {
+  const int form = kFwdRelBias | (prm.ex.bias != nullptr ? kFwdVecBias : 0) | (prm.ex.dropout ? kFwdDropout : 0);
+#define FO_REL_FORM(M)                                                                                                \
+  if (form == (M)) {                                                                                                  \
+    if (prm.d_real > 64)                                                                                              \
+      return bf16 ? launch_ws64r<128, true, (M)>(tq, tk, tv, prm, stream) : launch_ws64r<128, false, (M)>(tq, tk, tv, prm, stream); \
+    return bf16 ? launch_ws64r<64, true, (M)>(tq, tk, tv, prm, stream) : launch_ws64r<64, false, (M)>(tq, tk, tv, prm, stream);     \
+  }
+  FO_REL_FORM(kFwdRelBias)
+  FO_REL_FORM(kFwdRelBias | kFwdVecBias)
+  FO_REL_FORM(kFwdRelBias | kFwdDropout)
+  FO_REL_FORM(kFwdRelBias | kFwdVecBias | kFwdDropout)
+#undef FO_REL_FORM
+  return fail(FO_ERR_UNSUPPORTED, "no kernel of this form");
+}
+
+int launch_bwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
+                   const CUtensorMap& tdq, const AttnBwdParams& prm, bool bf16, cudaStream_t stream) {
+#define FO_REL_FORM(DK, M) \
+  bf16 ? launch_bwd<DK, true, (M)>(tq, tk, tv, tdo, tdq, prm, stream) : launch_bwd<DK, false, (M)>(tq, tk, tv, tdo, tdq, prm, stream)
+  if (prm.d_real > 64) {
+    if (prm.ex.dropout) return FO_REL_FORM(128, kBwdRelBias | kBwdDropout);
+    return FO_REL_FORM(128, kBwdRelBias);
+  }
+  if (prm.ex.dropout) return FO_REL_FORM(64, kBwdRelBias | kBwdDropout);
+  return FO_REL_FORM(64, kBwdRelBias);
+#undef FO_REL_FORM
+}
+
+int launch_decode_rel(const DecodeParams& prm, const RelArgs& args, const AttnExtras& ex, int B, int H, int Sk, int D,
+                      bool shared_kv, bool bf16, int num_sms, int device, cudaStream_t stream) {
+  DecodeRel rel;
+  rel.buckets = args.buckets;
+  rel.table = static_cast<const uint8_t*>(args.table);
+  rel.stride_bucket = args.stride_bucket;
+  rel.stride_head = args.stride_head;
+  rel.table_f32 = args.table_f32;
+  rel.offset = args.bias.offset;
+  rel.bias = static_cast<const uint8_t*>(ex.bias);
+  rel.bias_stride_b = ex.bias_stride_b;
+  rel.bias_stride_h = ex.bias_stride_h;
+  rel.bias_f32 = ex.bias_f32;
+  const DecodeShape shape = decode_shape(B, H, Sk, D, shared_kv, num_sms);
+#define FO_DECODE(DK, HEADS, WARPS)                                                                                     \
+  if ((DK == 64) == (D <= 64) && shape.heads == HEADS && shape.warps == WARPS)                                          \
+    return bf16 ? launch_decode<DK, true, HEADS, WARPS>(prm, rel, B, shape.split, num_sms, device, stream)              \
+                : launch_decode<DK, false, HEADS, WARPS>(prm, rel, B, shape.split, num_sms, device, stream);
+#define FO_DECODE_WARPS(DK, HEADS) FO_DECODE(DK, HEADS, 8) FO_DECODE(DK, HEADS, 4) FO_DECODE(DK, HEADS, 2)
+  FO_DECODE_WARPS(64, 1)
+  FO_DECODE_WARPS(64, 4)
+  FO_DECODE_WARPS(128, 1)
+  FO_DECODE_WARPS(128, 4)
+#undef FO_DECODE_WARPS
+#undef FO_DECODE
+  return fail(FO_ERR_UNSUPPORTED, "no decoding kernel of this shape");
+}
+
+}  // namespace fo
+
+extern "C" int64_t fo_rel_attn_workspace(int H, int Sq, int Sk, const int* starts, int n_starts, int two_sided,
+                                         int query_offset) {
+  fo::clear_error();
+  RelArgs rel;
+  const int64_t strides[2] = {0, 0};
+  const float table = 0;
+  if (make_rel_args(&rel, Sq, Sk, &table, FO_F32, strides, starts, n_starts, two_sided, query_offset, FO_BF16)) return -1;
+  if (H <= 0) {
+    fo::fail(FO_ERR_INVALID_ARGUMENT, "H must be positive (got %d)", H);
+    return -1;
+  }
+  return expanded_bytes(rel.bias, H);
+}
+
+extern "C" int64_t fo_rel_attn_bwd_workspace(int B, int H, int Sq, int Sk, int D, int num_buckets, int dropout) {
+  fo::clear_error();
+  if (B <= 0 || H <= 0 || Sq <= 0 || Sk <= 0 || D <= 0 || num_buckets <= 0) {
+    fo::fail(FO_ERR_INVALID_ARGUMENT, "B, H, Sq, Sk, D and num_buckets must be positive");
+    return -1;
+  }
+  return (tile_sum_floats(B, H, Sq, Sk, D, dropout != 0) + bucket_sum_floats(B, H, Sk, D, num_buckets, dropout != 0)) * 4;
+}
+
+extern "C" int fo_rel_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
+                               int B, int H, int Sq, int Sk, int D,
+                               const int64_t q_strides[3], const int64_t k_strides[3],
+                               const int64_t v_strides[3], const int64_t o_strides[3],
+                               int dtype, int causal, float softmax_scale,
+                               const void* table, const int64_t table_strides[2], int table_dtype,
+                               const int* starts, int n_starts, int two_sided, int query_offset, void* workspace,
+                               const void* bias, const int64_t bias_strides[3], int bias_dtype,
+                               float dropout_p, uint64_t rng_seed, uint64_t rng_offset,
+                               int device, void* stream) {
+  fo::clear_error();
+  RelArgs rel;
+  if (int rc = make_rel_args(&rel, Sq, Sk, table, table_dtype, table_strides, starts, n_starts, two_sided, query_offset, dtype))
+    return rc;
+  FO_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0, "workspace must be given, 4-byte aligned");
+  FO_REQUIRE(H > 0, "H must be positive (got %d)", H);
+  if (int rc = check_bias_strides(bias, bias_strides)) return rc;
+  fo::AttnExtras ex;
+  if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset)) return rc;
+  set_expanded(&rel.bias, workspace, H);
+  return fo::attn_fwd_impl(q, k, v, o, lse, B, H, Sq, Sk, D, q_strides, k_strides, v_strides, o_strides, dtype, causal,
+                           softmax_scale, &ex, &rel, device, stream);
+}
+
+extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                               const float* lse, void* dq, void* dk, void* dv, void* dtable, float* dq_accum, float* delta,
+                               float* partials, int B, int H, int Sq, int Sk, int D,
+                               const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                               const int64_t o_strides[3], const int64_t do_strides[3],
+                               const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3],
+                               int dtype, int causal, float softmax_scale, int table_dtype,
+                               const int* starts, int n_starts, int two_sided, int query_offset, const void* workspace,
+                               const void* bias, const int64_t bias_strides[3], int bias_dtype,
+                               float dropout_p, uint64_t rng_seed, uint64_t rng_offset,
+                               int device, void* stream) {
+  fo::clear_error();
+  RelArgs rel;
+  const int64_t no_strides[2] = {0, 0};
+  // the table itself is not read again: its expanded form is
+  if (int rc = make_rel_args(&rel, Sq, Sk, workspace, table_dtype, no_strides, starts, n_starts, two_sided, query_offset, dtype))
+    return rc;
+  FO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 3) == 0, "workspace must be 4-byte aligned");
+  FO_REQUIRE(H > 0 && B > 0, "B and H must be positive (got %d %d)", B, H);
+  FO_REQUIRE(dtable == nullptr || partials != nullptr, "the table's gradient needs its workspace");
+  FO_REQUIRE((reinterpret_cast<uintptr_t>(partials) & 7) == 0, "partials must be 8-byte aligned");
+  FO_REQUIRE(reinterpret_cast<uintptr_t>(dtable) % (table_dtype == FO_F32 ? 4 : 2) == 0, "dtable is not aligned to its elements");
+  if (int rc = check_bias_strides(bias, bias_strides)) return rc;
+  fo::AttnExtras ex;
+  if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset)) return rc;
+  set_expanded(&rel.bias, const_cast<void*>(workspace), H);
+  if (dtable != nullptr) {
+    rel.bias.tile_sums = reinterpret_cast<float2*>(partials);
+    rel.bias.acc = partials + tile_sum_floats(B, H, Sq, Sk, D, ex.dropout != 0);
+  }
+  if (int rc = fo::attn_bwd_impl(q, k, v, o, dout, lse, dq, dk, dv, dq_accum, delta, B, H, Sq, Sk, D, q_strides, k_strides,
+                                 v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, dtype, causal,
+                                 softmax_scale, &ex, &rel, device, stream))
+    return rc;
+  if (dtable == nullptr) return FO_OK;
+  fo::DeviceGuard guard(device);
+  FO_REQUIRE(guard.ok, "cannot make device %d current", device);
+  const int q_tiles = (Sq + fo::kBlockM - 1) / fo::kBlockM, k_tiles = (Sk + fo::kBlockN - 1) / fo::kBlockN;
+  const int warps = bwd_warps(D, ex.dropout != 0);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const float inv = 1.f / softmax_scale;
+#define FO_TABLE_GRAD(T)                                                                                             \
+  rel_table_grad_kernel<<<H, 1024, 0, s>>>(rel.bias, static_cast<T*>(dtable), B, H, q_tiles, k_tiles, warps, causal ? 1 : 0, inv)
+  if (table_dtype == FO_F32) FO_TABLE_GRAD(float);
+  else if (table_dtype == FO_BF16) FO_TABLE_GRAD(__nv_bfloat16);
+  else FO_TABLE_GRAD(__half);
+#undef FO_TABLE_GRAD
+  fo::g_launch_count.fetch_add(1, std::memory_order_relaxed);
+  FO_CUDA_CHECK(cudaGetLastError());
+  return FO_OK;
+}

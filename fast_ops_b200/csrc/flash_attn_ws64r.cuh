@@ -22,7 +22,8 @@
 
 namespace fo {
 
-// kExt: kFwdVecBias, kFwdMatBias or kFwdMatBias32, with or without kFwdDropout.
+// kExt: kFwdVecBias, kFwdMatBias, kFwdMatBias32 or kFwdRelBias with or without kFwdVecBias, and
+// kFwdDropout with any of them.
 template <int D, bool kBf16, int kExt>
 __global__ void __launch_bounds__(512, 1)
 attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -89,8 +90,10 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   const int h = bh - b * prm.H;
   const int hk = prm.kv_head_bcast ? 0 : h;  // head coordinate of K and V
   // keys visible to query tile 0 / 1 of this pair, in 64-key steps (T) and 128-key tiles (n)
-  const int vis0 = prm.causal ? min(prm.Sk, (2 * pair + 1) * kBlockM) : prm.Sk;
-  const int vis1 = prm.causal ? min(prm.Sk, (2 * pair + 2) * kBlockM) : prm.Sk;
+  constexpr bool rel_bias = (kExt & kFwdRelBias) != 0;
+  const int q_off = rel_bias ? prm.rel.offset : 0;  // query row i stands at key position i + q_off
+  const int vis0 = prm.causal ? min(prm.Sk, (2 * pair + 1) * kBlockM + q_off) : prm.Sk;
+  const int vis1 = prm.causal ? min(prm.Sk, (2 * pair + 2) * kBlockM + q_off) : prm.Sk;
   const int n0 = (vis0 + kBlockN - 1) / kBlockN;
   const int n1 = (vis1 + kBlockN - 1) / kBlockN;
   const int T0 = 2 * n0, T1 = 2 * n1;  // T1 >= T0 >= 2
@@ -108,11 +111,18 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     float bias_first = 0.f, bias_last = 0.f;
     if (n1 > 1) {
       const int64_t row = min((2 * pair + 1) * kBlockM, prm.Sq - 1);
-      const uint8_t* const p = static_cast<const uint8_t*>(prm.ex.bias) +
-                               (b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h + row * prm.ex.bias_stride_q) *
-                                   (prm.ex.bias_f32 ? 4 : 2);
-      bias_first = load_bias1<kBf16>(prm.ex, p, 0);
-      bias_last = load_bias1<kBf16>(prm.ex, p, vis0 - 1);
+      if constexpr ((kExt & ~(kFwdRelBias | kFwdDropout)) != 0) {
+        const uint8_t* const p = static_cast<const uint8_t*>(prm.ex.bias) +
+                                 (b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h + row * prm.ex.bias_stride_q) *
+                                     (prm.ex.bias_f32 ? 4 : 2);
+        bias_first = load_bias1<kBf16>(prm.ex, p, 0);
+        bias_last = load_bias1<kBf16>(prm.ex, p, vis0 - 1);
+      }
+      if constexpr (rel_bias) {
+        const int d0 = -static_cast<int>(row) - q_off;  // relative position of key 0
+        bias_first += rel_value(prm.rel, h, d0);
+        bias_last += rel_value(prm.rel, h, d0 + vis0 - 1);
+      }
     }
     const int status = *reinterpret_cast<volatile int*>(prm.device_status);
     mbar_init(bar_q_full, 1);
@@ -221,11 +231,25 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const uint8_t* bias_vec = nullptr;
     float* sb = s_bias + s * 256;
     float bias_next = 0.f;
+    // a relative bias: this row's values by key (read only near the diagonal), and the two far constants
+    const float* rel_row = nullptr;
+    float rel_left = 0.f, rel_right = 0.f;
+    const int warp_row = q0 + (warp & 3) * 32 + q_off;  // key position of the warp's first row
+    if constexpr (rel_bias) {
+      rel_row = prm.rel.values + static_cast<int64_t>(h) * prm.rel.width;
+      rel_left = __ldg(rel_row);
+      rel_right = __ldg(rel_row + prm.rel.width - 1);
+      rel_row += static_cast<int64_t>(prm.rel.zero) - row - q_off;
+    }
+    auto load_vec = [&](int col) {
+      if constexpr (rel_bias) return scaled_or_masked(load_elem<kBf16>(bias_vec, col, prm.ex.bias_f32));
+      else return load_bias1<kBf16>(prm.ex, bias_vec, col);
+    };
     if constexpr (vec_bias) {
       bias_vec = static_cast<const uint8_t*>(prm.ex.bias) +
                  (b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h) * (prm.ex.bias_f32 ? 4 : 2);
       const int col = key0 + r;
-      bias_next = (col < prm.Sk) ? load_bias1<kBf16>(prm.ex, bias_vec, col) : 0.f;
+      bias_next = (col < prm.Sk) ? load_vec(col) : 0.f;
     }
 
     // S of the next step is normally complete long before it is needed: polled once while the
@@ -252,7 +276,7 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       const int j = tn >> 1;
       sb[(j & 1) * 128 + r] = bias_next;
       const int col = key0 + (j + 1) * tile_dir + r;  // of the key tile after this one (there may be none)
-      bias_next = (col >= 0 && col < prm.Sk) ? load_bias1<kBf16>(prm.ex, bias_vec, col) : 0.f;
+      bias_next = (col >= 0 && col < prm.Sk) ? load_vec(col) : 0.f;
       // a buffer is rewritten two key tiles later, behind the barrier of the tile between
       named_barrier_sync(1 + s, 128);
     };
@@ -284,12 +308,38 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     // Waits for those loads and applies bias and masks in place.
     auto prep_loads = [&](int tn) {
       const int k0n = step_key(tn, first, key0);
-      const bool need_mask = (k0n + kStepN > prm.Sk) || (prm.causal && k0n + kStepN - 1 > q0);
+      const bool need_mask = (k0n + kStepN > prm.Sk) || (prm.causal && k0n + kStepN - 1 > q0 + q_off);
+      // relative positions of the warp's 32 rows and the step's keys: d_last - 94 to d_last
+      const int d_last = k0n + kStepN - 1 - warp_row;
+      const bool rel_near = rel_bias && d_last > -prm.rel.far_left && d_last - (kStepN + 30) < prm.rel.far_right;
+      const float rel_far = d_last > -prm.rel.far_left ? rel_right : rel_left;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         tmem_ld_wait(sr[c]);
         if ((warp & 3) == 0 && tn > 0) trace_event(prm, s, tn - 1, c == 0 ? 1 : 4);  // loads in
-        if constexpr (vec_bias) {
+        if constexpr (rel_bias) {
+          const float4* bv = reinterpret_cast<const float4*>(sb + ((tn >> 1) & 1) * 128 + ((tn & 1) ^ first) * kStepN + c * 32);
+          if (rel_near) {
+            float bb[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) bb[i] = __ldg(rel_row + k0n + c * 32 + i);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float4 v4 = make_float4(0.f, 0.f, 0.f, 0.f);
+              if constexpr (vec_bias) v4 = bv[i >> 2];
+              add_bias2(c, i, make_float2(bb[i] + v4.x, bb[i + 1] + v4.y));
+              add_bias2(c, i + 2, make_float2(bb[i + 2] + v4.z, bb[i + 3] + v4.w));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              float4 v4 = make_float4(0.f, 0.f, 0.f, 0.f);
+              if constexpr (vec_bias) v4 = bv[i >> 2];
+              add_bias2(c, i, make_float2(rel_far + v4.x, rel_far + v4.y));
+              add_bias2(c, i + 2, make_float2(rel_far + v4.z, rel_far + v4.w));
+            }
+          }
+        } else if constexpr (vec_bias) {
           const float4* bv = reinterpret_cast<const float4*>(sb + ((tn >> 1) & 1) * 128 + ((tn & 1) ^ first) * kStepN + c * 32);
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
@@ -323,7 +373,7 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int col = k0n + c * 32 + i;
-            if (col >= prm.Sk || (prm.causal && col > row)) sr[c][i] = 0xff800000u;  // -inf
+            if (col >= prm.Sk || (prm.causal && col > row + q_off)) sr[c][i] = 0xff800000u;  // -inf
           }
         }
       }

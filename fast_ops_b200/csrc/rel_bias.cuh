@@ -1,0 +1,72 @@
+// A learned relative position bias: the score of query i and key j gets table[bucket(j - i - offset)][head].
+//
+// Buckets are given by the smallest distance of each of them, `starts` (0 = starts[0] <= starts[1] ...): a
+// distance n lies in the last bucket whose start is not above n.  One-sided, n = max(i + offset - j, 0);
+// two-sided, n = |j - i - offset|, and the keys behind the query have a second set of buckets.
+//
+// The tile kernels read the bias of a head as a vector over the relative position d = j - i - offset, at
+// x = d + zero, times log2(e).  It is constant from -far_left down and from far_right up, so that only the
+// tiles near the diagonal read it at all; its ends reach kRelMargin further, which is more than a warp's
+// part of such a tile can.
+#pragma once
+
+#include <cstdint>
+
+namespace fo {
+
+constexpr int kRelMaxStarts = 256;  // buckets of one side: they travel in kernel arguments
+constexpr int kRelMargin = 192;
+
+struct RelBuckets {
+  int starts[kRelMaxStarts];
+  int n;          // buckets of one side
+  int two_sided;
+};
+
+__device__ __forceinline__ int rel_bucket(const RelBuckets& bk, int d) {
+  const int n = bk.two_sided ? abs(d) : max(-d, 0);
+  int lo = 0, hi = bk.n - 1;  // starts[lo] <= n, and nothing above hi is
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (bk.starts[mid] <= n) lo = mid;
+    else hi = mid - 1;
+  }
+  return bk.two_sided && d > 0 ? lo + bk.n : lo;
+}
+
+// A bias in the units of the exponent, log2(e) * value, where -1e6 and less masks as -inf does.  (Taken as a
+// number, a mask that leaves a row without keys would give it an LSE of that size, from which the backward
+// cannot tell P: at -1e9 the spacing of fp32 is 64, and P = exp(s - LSE) could be anything, infinity
+// included.  Rows with a key left do not change: e^-1e6 is 0.)
+__device__ __forceinline__ float scaled_or_masked(float v) {
+  return v <= -1e6f ? __int_as_float(0xff800000) : v * 1.4426950408889634f;
+}
+
+// What the tile kernels need; null `values`: no relative bias.
+struct RelBias {
+  const float* values;   // [H][width]
+  const int* bucket_of;  // [width]
+  // Backward, null without a gradient of the table: the tiles near the diagonal summed by bucket,
+  // [B*H][key tiles][warps][buckets], and the sums of dS and of P over each warp's part of every tile,
+  // [B*H][query tiles][key tiles][warps].
+  float* acc;
+  float2* tile_sums;
+  int width, zero;
+  int far_left, far_right;
+  int offset;
+  int num_buckets;
+};
+
+// Where a rectangle of scores lies whose relative positions go from `first` to `last`.
+enum RelSide { kRelNear = 0, kRelLeft = 1, kRelRight = 2 };
+__device__ __forceinline__ RelSide rel_side(const RelBias& rel, int first, int last) {
+  return last <= -rel.far_left ? kRelLeft : first >= rel.far_right ? kRelRight : kRelNear;
+}
+
+// Bias (times log2(e)) of relative position d for head h, whatever d is.
+__device__ __forceinline__ float rel_value(const RelBias& rel, int h, int d) {
+  const int x = min(max(d, -rel.zero), rel.width - 1 - rel.zero) + rel.zero;
+  return __ldg(rel.values + static_cast<int64_t>(h) * rel.width + x);
+}
+
+}  // namespace fo

@@ -8,3 +8,4 @@ from .flash_attention import (  # noqa: F401
 )
 from .flash_attention_bshd import flash_attn_bshd, triton_dropout_mask  # noqa: F401
 from .host import flash_attention_forward_host  # noqa: F401
+from .relative import relative_attention, relative_bucket_starts  # noqa: F401

@@ -1,0 +1,240 @@
+"""Attention with a learned relative position bias, differentiable in the bias.
+
+The bias of query i and key j is table[bucket(j - (i + query_offset)), head]: near positions have a
+bucket each, far ones share buckets that grow with the distance.  It is never materialised: the
+kernels read it as one vector per head, add a constant away from the diagonal, and sum the table's
+gradient where the backward forms dS.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from functools import lru_cache
+from typing import Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from .flash_attention import _CODES, _prepare_bias, _strides3, next_dropout_rng
+
+_I64x2 = ctypes.c_int64 * 2
+#: buckets of one side (the C ABI passes their starts in kernel arguments)
+MAX_BUCKETS_PER_SIDE = 256
+
+
+@lru_cache(maxsize=64)
+def relative_bucket_starts(num_buckets: int, max_distance: int, bidirectional: bool) -> Tuple[int, ...]:
+    """The smallest distance of each bucket of one side.
+
+    With h buckets on a side (half of `num_buckets` if bidirectional, otherwise all) and e = h // 2,
+    distances below e have a bucket each; bucket e + x starts at the smallest n with
+    (n / e)^(h - e) >= (max_distance / e)^x: equal steps of the logarithm, up to `max_distance`, decided
+    in whole numbers.  The last bucket takes everything beyond.  Positions after the query come
+    second, from bucket h on; one-sided, they all count as distance 0.
+    """
+    if num_buckets < 2 or (bidirectional and (num_buckets < 4 or num_buckets % 2)):
+        raise RuntimeError(f"num_buckets must be at least 2, or even and at least 4 if bidirectional, got {num_buckets}")
+    per_side = num_buckets // 2 if bidirectional else num_buckets
+    if per_side > MAX_BUCKETS_PER_SIDE:
+        raise RuntimeError(f"at most {MAX_BUCKETS_PER_SIDE} buckets per side, got {per_side}")
+    exact = per_side // 2
+    if not exact < max_distance < 2**29:
+        raise RuntimeError(f"max_distance must be above {exact} and below 2^29, got {max_distance}")
+    steps = per_side - exact
+    starts = list(range(exact))
+    for x in range(steps):
+        bound = max_distance**x * exact ** (steps - x)  # n^steps >= bound
+        n = max(starts[-1] if starts else 0, int(math.exp(math.log(max_distance / exact) * x / steps) * exact) - 2, exact)
+        while n**steps < bound:
+            n += 1
+        while n > exact and (n - 1) ** steps >= bound:
+            n -= 1
+        starts.append(n)
+    return tuple(starts)
+
+
+@lru_cache(maxsize=64)
+def _starts_array(num_buckets: int, max_distance: int, bidirectional: bool):
+    starts = relative_bucket_starts(num_buckets, max_distance, bidirectional)
+    return (ctypes.c_int * len(starts))(*starts), len(starts)
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(H: int, M: int, N: int, num_buckets: int, max_distance: int, bidirectional: bool, offset: int) -> int:
+    starts, n = _starts_array(num_buckets, max_distance, bidirectional)
+    size = _lib.load().fo_rel_attn_workspace(H, M, N, starts, n, int(bidirectional), offset)
+    _lib.check(-1 if size < 0 else 0)
+    return size
+
+
+class _Call:
+    """The checked arguments of one call, shared by forward and backward."""
+
+    def __init__(self, Q: Tensor, K: Tensor, V: Tensor, table: Tensor, max_distance: int, bidirectional: bool,
+                 query_offset: int, causal: bool, softmax_scale: Optional[float], dropout_p: float,
+                 rng: Optional[Tuple[int, int]]):
+        if not all(isinstance(t, Tensor) for t in (Q, K, V, table)):
+            raise RuntimeError("Q, K, V and table must be tensors")
+        if Q.dim() != 4 or K.dim() != 4 or V.dim() != 4:
+            raise RuntimeError("Q, K, V must be 4-D")
+        if not Q.is_cuda:
+            raise RuntimeError("fast_ops_b200 attention needs CUDA tensors (there is no CPU path)")
+        if any(t.device != Q.device for t in (K, V, table)):
+            raise RuntimeError("Q, K, V and table must be on the same device")
+        code = _CODES.get(Q.dtype)
+        if code is None:
+            raise RuntimeError(f"inputs must be float16 or bfloat16, got {Q.dtype}")
+        if K.dtype != Q.dtype or V.dtype != Q.dtype:
+            raise RuntimeError("Q, K, V must have the same dtype")
+        if table.dtype not in (Q.dtype, torch.float32):
+            raise RuntimeError(f"table must be float32 or have Q's dtype, got {table.dtype}")
+        B, H, M, D = Q.shape
+        if K.shape[:2] != (B, H) or K.shape[3] != D or V.shape != K.shape:
+            raise RuntimeError(f"shape mismatch: Q {tuple(Q.shape)}, K {tuple(K.shape)}, V {tuple(V.shape)}")
+        if table.dim() != 2 or table.shape[1] != H:
+            raise RuntimeError(f"table must be (num_buckets, {H}), got {tuple(table.shape)}")
+        if D > 128 or D % 8 != 0 or D == 0:
+            raise RuntimeError(f"head_dim must be a multiple of 8 and <= 128, got {D}")
+        for name, t in (("Q", Q), ("K", K), ("V", V)):
+            if t.stride(3) != 1:
+                raise RuntimeError(f"{name}: the last dimension must be contiguous")
+        if not 0.0 <= dropout_p < 1.0:
+            raise RuntimeError(f"dropout_p must be in [0, 1), got {dropout_p}")
+        if not 0 <= query_offset <= 2**29:
+            raise RuntimeError(f"query_offset must be in [0, 2^29], got {query_offset}")
+        self.B, self.H, self.M, self.D, self.N = B, H, M, D, K.shape[2]
+        self.code, self.device, self.index = code, Q.device, Q.get_device()
+        self.table_dtype = _lib.FO_F32 if table.dtype == torch.float32 else code
+        self.num_buckets = table.shape[0]
+        self.key = (self.num_buckets, int(max_distance), bool(bidirectional))
+        self.starts, self.n_starts = _starts_array(*self.key)
+        self.bidirectional, self.offset, self.causal = int(bool(bidirectional)), int(query_offset), int(bool(causal))
+        self.scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D)
+        self.dropout_p = float(dropout_p)
+        if self.dropout_p > 0.0 and rng is None:
+            rng = next_dropout_rng(Q.device, B * H * M * self.N)
+        self.rng = (0, 0) if rng is None else (rng[0] & (2**64 - 1), rng[1] & (2**64 - 1))
+
+    def bias(self, bias: Optional[Tensor], Q: Tensor):
+        if bias is not None and bias.dim() == 4 and bias.shape[2] != 1:
+            raise RuntimeError("beside a relative bias, bias must be (1 or B, 1 or H, 1, N): the same for every query")
+        kept, ptr, strides, code = _prepare_bias(bias, Q, self.B, self.H, self.M, self.N)
+        if strides is not None:
+            strides[2] = 0  # a single query row's stride says nothing
+        return kept, (ptr, strides, code)
+
+    def forward(self, Q: Tensor, K: Tensor, V: Tensor, table: Tensor, bias: Optional[Tensor], lse: bool):
+        """(O, LSE or None, the expanded bias)."""
+        O = torch.empty_like(Q, memory_format=torch.contiguous_format)
+        lse_t = Q.new_empty((self.B, self.H, self.M), dtype=torch.float32) if lse else None
+        workspace = torch.empty(_workspace_bytes(self.H, self.M, self.N, *self.key, self.offset), dtype=torch.uint8,
+                                device=self.device)
+        kept, bias_args = self.bias(bias, Q)
+        ts = table.stride()
+        _lib.check(_lib.load().fo_rel_attn_fwd(
+            Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), lse_t.data_ptr() if lse else None, self.B, self.H, self.M, self.N, self.D,
+            _strides3(Q), _strides3(K), _strides3(V), _strides3(O), self.code, self.causal, self.scale,
+            table.data_ptr(), _I64x2(ts[0], ts[1]), self.table_dtype, self.starts, self.n_starts, self.bidirectional,
+            self.offset, workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
+            _lib.current_stream_ptr(self.index)))
+        return O, lse_t, workspace
+
+    def backward(self, dO: Tensor, Q: Tensor, K: Tensor, V: Tensor, O: Tensor, LSE: Tensor, workspace: Tensor,
+                 bias: Optional[Tensor], table_grad: Optional[torch.dtype]):
+        """(dQ, dK, dV, the table's gradient or None)."""
+        if dO.stride(3) != 1:
+            dO = dO.contiguous()
+        if K.stride(1) == 0 or V.stride(1) == 0:
+            # one K/V head for all query heads: one dK, dV per query head needs storage of its own
+            # (autograd sums them through the expand)
+            K, V = K.contiguous(), V.contiguous()
+        dQ, dK, dV = torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V)
+        for t in (dQ, dK, dV):
+            if t.stride(3) != 1:
+                raise RuntimeError("gradient layout: the last dimension must be contiguous")
+        lib = _lib.load()
+        rows = self.B * self.H * self.M
+        partials = 0
+        dtable = None
+        if table_grad is not None:
+            dtable = torch.empty((self.num_buckets, self.H), dtype=table_grad, device=self.device)
+            partials = lib.fo_rel_attn_bwd_workspace(self.B, self.H, self.M, self.N, self.D, self.num_buckets,
+                                                     int(self.dropout_p > 0.0)) // 4
+        # one scratch block: the fp32 dQ accumulator (B, H, M, D), the table's partial sums, rowsum(O o dO) (B, H, M)
+        scratch = torch.empty(rows * (self.D + 1) + partials, dtype=torch.float32, device=self.device)
+        dq_accum = scratch.data_ptr()
+        partial_sums = dq_accum + 4 * rows * self.D  # a multiple of 32 bytes on, since D is one of 8
+        kept, bias_args = self.bias(bias, Q)
+        _lib.check(lib.fo_rel_attn_bwd(
+            Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), dO.data_ptr(), LSE.data_ptr(), dQ.data_ptr(),
+            dK.data_ptr(), dV.data_ptr(), None if dtable is None else dtable.data_ptr(), dq_accum,
+            partial_sums + 4 * partials, partial_sums,
+            self.B, self.H, self.M, self.N, self.D,
+            _strides3(Q), _strides3(K), _strides3(V), _strides3(O), _strides3(dO), _strides3(dQ), _strides3(dK),
+            _strides3(dV), self.code, self.causal, self.scale, self.table_dtype, self.starts, self.n_starts,
+            self.bidirectional, self.offset, workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
+            _lib.current_stream_ptr(self.index)))
+        return dQ, dK, dV, dtable
+
+
+class _RelativeAttentionFunction(Function):
+    @staticmethod
+    def forward(ctx, Q: Tensor, K: Tensor, V: Tensor, table: Tensor, call: _Call, bias: Optional[Tensor],
+                return_lse: bool):
+        O, lse, workspace = call.forward(Q, K, V, table, bias, True)
+        ctx.save_for_backward(Q, K, V, O, lse, workspace, bias)
+        ctx.call, ctx.table_dtype = call, table.dtype
+        if not return_lse:
+            return O
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(lse)
+        return O, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dO: Optional[Tensor], _dlse=None):
+        if dO is None:
+            return (None,) * 7
+        Q, K, V, O, lse, workspace, bias = ctx.saved_tensors
+        return ctx.call.backward(dO, Q, K, V, O, lse, workspace, bias,
+                                 ctx.table_dtype if ctx.needs_input_grad[3] else None) + (None,) * 3
+
+
+def relative_attention(Q: Tensor, K: Tensor, V: Tensor, table: Tensor, *, max_distance: int = 128,
+                       bidirectional: bool = True, query_offset: int = 0, causal: bool = False,
+                       softmax_scale: Optional[float] = None, return_lse: bool = False,
+                       bias: Optional[Tensor] = None, dropout_p: float = 0.0,
+                       rng: Optional[Tuple[int, int]] = None) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """softmax(scale * Q K^T + table[bucket(j - i - query_offset)] [+ bias] [+ causal mask]) V.
+
+    Q: (B, H, M, D); K, V: (B, H, N, D); fp16 or bf16, layouts as in `multi_head_attention` (K and V may
+    be expanded over the heads).  Differentiable in Q, K, V and `table`.
+
+    :param table: (num_buckets, H), fp32 or Q's dtype, any non-negative strides.
+    :param max_distance, bidirectional: the buckets, see `relative_bucket_starts`.  Bidirectional, keys
+        before and after the query have num_buckets / 2 buckets each; otherwise all buckets are for the
+        keys before it and those after it are at distance 0 (as a causal model wants it).
+    :param query_offset: key position of query row 0.  A decoder that has N keys stored and asks for the
+        last M of them passes N - M; a single query row runs in the decoding kernel.
+    :param causal: masks keys j > i + query_offset.
+    :param bias: added beside the learned bias, not differentiable: (1 or B, 1 or H, 1, N), fp32 or Q's
+        dtype; entries of -1e6 and below mask keys (padding), as -inf does.  A query row whose keys are
+        all masked gives zeros, and no gradients.
+    :param dropout_p, rng: as in `flash_attention_forward`; without `rng` the mask is drawn from the
+        device's default generator, as in `multi_head_attention`.
+    :returns: O (B, H, M, D), contiguous, or (O, LSE) with `return_lse`.
+
+    Violations of these raise RuntimeError.  The table's gradient is summed in an order that does not
+    change from run to run.
+    """
+    call = _Call(Q, K, V, table, max_distance, bidirectional, query_offset, causal, softmax_scale, dropout_p, rng)
+    if torch.is_grad_enabled():
+        if bias is not None and bias.requires_grad:
+            raise RuntimeError("the gradient of bias is not supported (that of table is)")
+        if Q.requires_grad or K.requires_grad or V.requires_grad or table.requires_grad:
+            return _RelativeAttentionFunction.apply(Q, K, V, table, call, bias, return_lse)
+    O, lse, _ = call.forward(Q, K, V, table, bias, return_lse)
+    return (O, lse) if return_lse else O

@@ -147,6 +147,52 @@ int fo_flash_attn_bwd_ex(const void* q, const void* k, const void* v, const void
                          int device, void* stream);
 
 /*
+ * Attention with a learned relative position bias: as fo_flash_attn_fwd_ex / fo_flash_attn_bwd_ex, with
+ *   s(i, j) = softmax_scale * q_i . k_j + table[bucket(j - i - query_offset)][h] [+ bias(b, h, j)],
+ * causal masking j > i + query_offset, and the gradient of the table.  The reference has no counterpart.
+ *
+ *   starts, n_starts, two_sided : the buckets (HOST array): a distance n lies in the last bucket u with
+ *                starts[u] <= n; starts[0] = 0, not descending, at most 256.  One-sided
+ *                (two_sided = 0), n = max(i + query_offset - j, 0); two-sided, n = |j - i - query_offset|
+ *                and keys behind the query take buckets n_starts + u.
+ *   table      : device pointer, fp32 or the dtype of q (table_dtype), element (bucket, head) at
+ *                table + bucket*s[0] + head*s[1] with s = table_strides in elements (non-negative).
+ *   query_offset : key position of query row 0, in [0, 2^29].
+ *   workspace  : device memory of fo_rel_attn_workspace(...) bytes, 4-byte aligned.  The forward writes
+ *                the expanded bias there; the backward must be given it as the forward left it.
+ *   bias       : as in fo_flash_attn_fwd_ex, but the same for every query row: bias_strides[2] = 0.
+ *                Entries of -1e6 and below mask like -inf, in the table too.
+ *   dtable     : NULL (no gradient of the table), or (n_buckets, H) dense, of table_dtype.
+ *   partials   : for dtable: fo_rel_attn_bwd_workspace(...) bytes of scratch, 8-byte aligned (`dropout`:
+ *                whether dropout_p > 0; num_buckets: n_starts, twice that if two-sided).
+ *
+ * Sq = 1 without dropout runs in the decoding kernel, which fills the workspace only if
+ * there is an lse (a backward may follow).
+ * The workspace functions return -1 for arguments that the calls refuse.
+ */
+int64_t fo_rel_attn_workspace(int H, int Sq, int Sk, const int* starts, int n_starts, int two_sided, int query_offset);
+int64_t fo_rel_attn_bwd_workspace(int B, int H, int Sq, int Sk, int D, int num_buckets, int dropout);
+int fo_rel_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
+                    int B, int H, int Sq, int Sk, int D,
+                    const int64_t q_strides[3], const int64_t k_strides[3],
+                    const int64_t v_strides[3], const int64_t o_strides[3],
+                    int dtype, int causal, float softmax_scale,
+                    const void* table, const int64_t table_strides[2], int table_dtype,
+                    const int* starts, int n_starts, int two_sided, int query_offset, void* workspace,
+                    const void* bias, const int64_t bias_strides[3], int bias_dtype,
+                    float dropout_p, uint64_t rng_seed, uint64_t rng_offset, int device, void* stream);
+int fo_rel_attn_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout,
+                    const float* lse, void* dq, void* dk, void* dv, void* dtable, float* dq_accum, float* delta,
+                    float* partials, int B, int H, int Sq, int Sk, int D,
+                    const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                    const int64_t o_strides[3], const int64_t do_strides[3],
+                    const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3],
+                    int dtype, int causal, float softmax_scale, int table_dtype,
+                    const int* starts, int n_starts, int two_sided, int query_offset, const void* workspace,
+                    const void* bias, const int64_t bias_strides[3], int bias_dtype,
+                    float dropout_p, uint64_t rng_seed, uint64_t rng_offset, int device, void* stream);
+
+/*
  * Materialises the keep mask of the dropout above as B*H*Sq*Sk bytes (1 = kept), dense in
  * (b, h, i, j) order.  Replaces triton_dropout_mask / _dropout_mask_kernel
  * (fast_ops/flash_attention/flash_attention_triton.py:668-717), which the reference's tests use
