@@ -41,6 +41,8 @@
 // columns each (in the epilogue two for dK, two for dV), and the other roles in warps 16 to 22.
 #pragma once
 
+#include <type_traits>
+
 #include "flash_attn_common.cuh"
 #include "fo_host.h"
 
@@ -344,17 +346,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     }
     // A relative bias: its values for this key by query row (read only near the diagonal), and the two far
     // constants.
-    const float* rel_col = nullptr;
+    const float4* rel_col = nullptr;
     float rel_left = 0.f, rel_right = 0.f;
     float* rel_acc = nullptr;
     float2* rel_sums = nullptr;  // of query tile 0
     const int64_t rel_sums_step = static_cast<int64_t>(gridDim.x) * kCW;
     const int warp_key = k0 + (warp & 3) * 32 - q_off;  // query row that the warp's first key stands beside
     if constexpr (rel_bias) {
-      rel_col = prm.rel.values + static_cast<int64_t>(h) * prm.rel.width;
-      rel_left = __ldg(rel_col);
-      rel_right = __ldg(rel_col + prm.rel.width - 1);
-      rel_col += static_cast<int64_t>(prm.rel.zero) + key - q_off;
+      rel_left = rel_value(prm.rel, h, -prm.rel.zero);
+      rel_right = rel_value(prm.rel, h, prm.rel.width);
+      // values of query rows 3 to 0, which may lie behind the vector; those read do not
+      const int x = prm.rel.zero + key - q_off - 3, s4 = x & 3;
+      rel_col = rel_vector(prm.rel, h, s4) + ((x - s4) >> 2);
       if (prm.ex.bias != nullptr && key_ok)
         bias_key = scaled_or_masked(load_elem<kBf16>(static_cast<const uint8_t*>(prm.ex.bias),
                                                      b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h + key, prm.ex.bias_f32));
@@ -397,15 +400,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         load_bias_rows32<kBf16>(prm.ex, bias_col + static_cast<int64_t>(q) * prm.ex.bias_stride_q * (prm.ex.bias_f32 ? 4 : 2),
                                 prm.Sq - q, bias_v);
       };
-      auto load_rel_piece = [&](int cc) {  // near the diagonal: this key's bias for 32 consecutive query rows
-        const float* const p = rel_col - (qc0 + cc * 32);
-#pragma unroll
-        for (int x = 0; x < 32; ++x) bias_v[x] = __ldg(p - x) + bias_key;
-      };
       if constexpr (mat_bias) load_bias_piece(0);
-      if constexpr (rel_bias) {
-        if (rel_near) load_rel_piece(0);
-      }
       const float rel_far = bias_key + (side == kRelLeft ? rel_left : rel_right);
       mbar_wait(bar_lse_full + Cfg::par(it), Cfg::phase(it), cta_abort, dstat, FO_STATUS_TIMEOUT_TMA);
       mbar_wait(bar_s_full, it & 1, cta_abort, dstat, FO_STATUS_TIMEOUT_MMA);
@@ -415,43 +410,66 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       uint32_t sr[kPieces][32];
 #pragma unroll
       for (int cc = 0; cc < kPieces; ++cc) tmem_ld32(tS + cc * 32, sr[cc]);
+      // with a relative bias the parts near the diagonal have a loop of their own
+      auto exponentials = [&](auto near) {
 #pragma unroll
-      for (int cc = 0; cc < kPieces; ++cc) {
-        const float* nl = sNegLse + (it & (Cfg::kSlots - 1)) * 128 + part * kCols + cc * 32;
-        tmem_ld_wait(sr[cc]);
-        if constexpr (mat_bias) {
-          if (cc > 0) load_bias_piece(cc);
-        }
-        if constexpr (rel_bias) {
-          if (rel_near && cc > 0) load_rel_piece(cc);
-          if (!rel_near) {
+        for (int cc = 0; cc < kPieces; ++cc) {
+          const float* nl = sNegLse + (it & (Cfg::kSlots - 1)) * 128 + part * kCols + cc * 32;
+          tmem_ld_wait(sr[cc]);
+          if constexpr (mat_bias) {
+            if (cc > 0) load_bias_piece(cc);
+          }
+          // this key's bias for 32 consecutive query rows, four at a time in descending order
+          const float4* const rv = rel_col - ((qc0 + cc * 32) >> 2);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) bias_v[x] = rel_far;
+          for (int x = 0; x < 32; x += 4) {
+            const float4 t = *reinterpret_cast<const float4*>(nl + x);  // broadcast read
+            const float nlv[4] = {t.x, t.y, t.z, t.w};
+            float bv[4] = {};
+            if constexpr (near.value) {
+              const float4 u = __ldg(rv - (x >> 2));
+              bv[0] = u.w + bias_key; bv[1] = u.z + bias_key; bv[2] = u.y + bias_key; bv[3] = u.x + bias_key;
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float sv = __uint_as_float(sr[cc][x + y]);
+              float e;
+              if constexpr (mat_bias) e = fmaf(sv, prm.scale_log2, bias_v[x + y]) + nlv[y];
+              else if constexpr (near.value) e = fmaf(sv, prm.scale_log2, bv[y]) + nlv[y];
+              else if constexpr (rel_bias) e = fmaf(sv, prm.scale_log2, rel_far) + nlv[y];
+              else if constexpr (vec_bias) e = fmaf(sv, prm.scale_log2, bias_key) + nlv[y];
+              else e = fmaf(sv, prm.scale_log2, nlv[y]);
+              sr[cc][x + y] = __float_as_uint(fast_exp2(e));
+            }
+          }
+          if (need_mask) {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+              const int q = qc0 + cc * 32 + x;
+              if (!key_ok || (prm.causal && key > q + q_off)) sr[cc][x] = 0u;
+            }
           }
         }
-#pragma unroll
-        for (int x = 0; x < 32; x += 4) {
-          const float4 t = *reinterpret_cast<const float4*>(nl + x);  // broadcast read
-          const float nlv[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float sv = __uint_as_float(sr[cc][x + y]);
-            float e;
-            if constexpr (mat_bias || rel_bias) e = fmaf(sv, prm.scale_log2, bias_v[x + y]) + nlv[y];
-            else if constexpr (vec_bias) e = fmaf(sv, prm.scale_log2, bias_key) + nlv[y];
-            else e = fmaf(sv, prm.scale_log2, nlv[y]);
-            sr[cc][x + y] = __float_as_uint(fast_exp2(e));
-          }
-        }
-        if (need_mask) {
-#pragma unroll
-          for (int x = 0; x < 32; ++x) {
-            const int q = qc0 + cc * 32 + x;
-            if (!key_ok || (prm.causal && key > q + q_off)) sr[cc][x] = 0u;
-          }
-        }
+      };
+      if constexpr (rel_bias) {
+        if (rel_near) exponentials(std::true_type{});
+        else exponentials(std::false_type{});
+      } else {
+        exponentials(std::false_type{});
       }
       if (warp == 0) bwd_trace(prm, 0, it, 4);
+      float p_sum = 0.f;
+      if constexpr (rel_bias) {
+        if (rel_acc != nullptr) {
+          float2 p2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int cc = 0; cc < kPieces; ++cc)
+#pragma unroll
+            for (int x = 0; x < 32; x += 2)
+              p2 = __fadd2_rn(p2, make_float2(__uint_as_float(sr[cc][x]), __uint_as_float(sr[cc][x + 1])));
+          p_sum = p2.x + p2.y;
+        }
+      }
       // ---- P^T (zero where the forward dropped the element), 16-bit, over the first half of this thread's S^T columns ----
       uint32_t pp[kPieces * 16];
 #pragma unroll
@@ -491,40 +509,46 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         float2 far_sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int k = 0; k <= kPieces; ++k) diag[k] = 0.f;
+        auto ds_columns = [&](auto diagonals) {
 #pragma unroll
-        for (int cc = 0; cc < kPieces; ++cc) {
-          const float* nd = sNegDelta + (it & (Cfg::kSlots - 1)) * 128 + part * kCols + cc * 32;
-          uint32_t dpr[32];
-          tmem_ld32(tDP + cc * 32, dpr);
-          tmem_ld_wait(dpr);
+          for (int cc = 0; cc < kPieces; ++cc) {
+            const float* nd = sNegDelta + (it & (Cfg::kSlots - 1)) * 128 + part * kCols + cc * 32;
+            uint32_t dpr[32];
+            tmem_ld32(tDP + cc * 32, dpr);
+            tmem_ld_wait(dpr);
 #pragma unroll
-          for (int x = 0; x < 32; x += 4) {
-            const float4 t = *reinterpret_cast<const float4*>(nd + x);  // broadcast read
-            const float ndv[4] = {t.x, t.y, t.z, t.w};
-            float dsv[4];
+            for (int x = 0; x < 32; x += 4) {
+              const float4 t = *reinterpret_cast<const float4*>(nd + x);  // broadcast read
+              const float ndv[4] = {t.x, t.y, t.z, t.w};
+              float dsv[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              float g = __uint_as_float(dpr[x + y]);
-              if constexpr (has_drop) {
-                if (!((keep[cc] >> (x + y)) & 1u)) g = 0.f;
+              for (int y = 0; y < 4; ++y) {
+                float g = __uint_as_float(dpr[x + y]);
+                if constexpr (has_drop) {
+                  if (!((keep[cc] >> (x + y)) & 1u)) g = 0.f;
+                }
+                dsv[y] = __uint_as_float(sr[cc][x + y]) * fmaf(g, dp_scale, ndv[y]);
               }
-              dsv[y] = __uint_as_float(sr[cc][x + y]) * fmaf(g, dp_scale, ndv[y]);
-            }
-            if constexpr (rel_bias) {
-              if (diag_sums) {
+              if constexpr (diagonals.value) {
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                   const float v = __shfl_sync(0xffffffffu, dsv[y], (lane + x + y) & 31);
                   if (lane + x + y < 32) diag[cc] += v;
                   else diag[cc + 1] += v;
                 }
-              } else {
+              } else if constexpr (rel_bias) {
                 far_sum = __fadd2_rn(far_sum, __fadd2_rn(make_float2(dsv[0], dsv[1]), make_float2(dsv[2], dsv[3])));
               }
+              dd[cc * 16 + (x >> 1)] = pack2<kBf16>(dsv[0], dsv[1]);
+              dd[cc * 16 + (x >> 1) + 1] = pack2<kBf16>(dsv[2], dsv[3]);
             }
-            dd[cc * 16 + (x >> 1)] = pack2<kBf16>(dsv[0], dsv[1]);
-            dd[cc * 16 + (x >> 1) + 1] = pack2<kBf16>(dsv[2], dsv[3]);
           }
+        };
+        if constexpr (rel_bias) {
+          if (diag_sums) ds_columns(std::true_type{});
+          else ds_columns(std::false_type{});
+        } else {
+          ds_columns(std::false_type{});
         }
         tmem_st_packed(tDP, dd);
 #pragma unroll
@@ -537,7 +561,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (warp == 0) bwd_trace(prm, 0, it, 1);
         if constexpr (rel_bias) {
           if (rel_acc != nullptr) {
-            float ds_sum = far_sum.x + far_sum.y, p_sum = 0.f;
+            float ds_sum = far_sum.x + far_sum.y;
             if (diag_sums) {
 #pragma unroll
               for (int k = 0; k <= kPieces; ++k) {
@@ -545,19 +569,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 add_diagonals(prm.rel, rel_acc, d_first + kCols - 1 + lane - 32 * k, lane, diag[k]);
               }
             }
-            float2 p2 = make_float2(0.f, 0.f);
+            // both sums over the warp: the lower half of the lanes goes on with dS, the upper with P
+            float sum = lane < 16 ? ds_sum : p_sum;
+            sum += __shfl_xor_sync(0xffffffffu, lane < 16 ? p_sum : ds_sum, 16);
 #pragma unroll
-            for (int cc = 0; cc < kPieces; ++cc)
-#pragma unroll
-              for (int x = 0; x < 32; x += 2)
-                p2 = __fadd2_rn(p2, make_float2(__uint_as_float(sr[cc][x]), __uint_as_float(sr[cc][x + 1])));
-            p_sum = p2.x + p2.y;
-#pragma unroll
-            for (int off = 16; off >= 1; off >>= 1) {
-              ds_sum += __shfl_xor_sync(0xffffffffu, ds_sum, off);
-              p_sum += __shfl_xor_sync(0xffffffffu, p_sum, off);
-            }
-            if (lane == 0) rel_sums[i * rel_sums_step] = make_float2(ds_sum, p_sum);
+            for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if ((lane & 15) == 0) reinterpret_cast<float*>(rel_sums + i * rel_sums_step)[lane >> 4] = sum;
           }
         }
       }

@@ -17,18 +17,20 @@ using fo::RelArgs;
 using fo::RelBias;
 using fo::RelBuckets;
 
-// values[h][x] = log2(e) * table[bucket(x - zero)][h], and the buckets themselves.
+// values[h][s][x] = log2(e) * table[bucket(x + s - zero)][h], and the buckets themselves.
 template <bool kBf16>
 __global__ void __launch_bounds__(256)
 rel_expand_kernel(const __grid_constant__ RelBuckets buckets, const uint8_t* __restrict__ table, int64_t stride_bucket,
-                  int64_t stride_head, int table_f32, int zero, int width, float* __restrict__ values,
+                  int64_t stride_head, int table_f32, int zero, int width, int stride, float* __restrict__ values,
                   int* __restrict__ bucket_of) {
   const int x = blockIdx.x * 256 + threadIdx.x;
   const int h = blockIdx.y;
   if (x >= width) return;
   const int bucket = fo::rel_bucket(buckets, x - zero);
-  values[static_cast<int64_t>(h) * width + x] =
-      fo::scaled_or_masked(fo::load_elem<kBf16>(table, bucket * stride_bucket + h * stride_head, table_f32));
+  const float v = fo::scaled_or_masked(fo::load_elem<kBf16>(table, bucket * stride_bucket + h * stride_head, table_f32));
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    if (x >= s) values[(static_cast<int64_t>(h) * 4 + s) * stride + x - s] = v;
   if (h == 0) bucket_of[x] = bucket;
 }
 
@@ -160,14 +162,15 @@ int make_rel_args(RelArgs* rel, int Sq, int Sk, const void* table, int table_dty
   bias.far_right = two_sided ? std::min(std::max(last, 1), Sk) : 0;
   bias.zero = bias.far_left + fo::kRelMargin;
   bias.width = bias.zero + bias.far_right + fo::kRelMargin + 1;
+  bias.stride = (bias.width + 3) / 4 * 4;
   return FO_OK;
 }
 
-int64_t expanded_bytes(const RelBias& bias, int H) { return (static_cast<int64_t>(H) + 1) * bias.width * 4; }
+int64_t expanded_bytes(const RelBias& bias, int H) { return (static_cast<int64_t>(H) * 4 + 1) * bias.stride * 4; }
 
 void set_expanded(RelBias* bias, void* workspace, int H) {
   bias->values = static_cast<const float*>(workspace);
-  bias->bucket_of = reinterpret_cast<const int*>(bias->values + static_cast<int64_t>(H) * bias->width);
+  bias->bucket_of = reinterpret_cast<const int*>(bias->values + static_cast<int64_t>(H) * 4 * bias->stride);
 }
 
 // Warps of the backward that sum for the table's gradient, per key tile.
@@ -202,7 +205,7 @@ int launch_rel_expand(const RelArgs& rel, int H, bool bf16, cudaStream_t stream)
   const dim3 grid((rel.bias.width + 255) / 256, H);
   auto kernel = bf16 ? rel_expand_kernel<true> : rel_expand_kernel<false>;
   kernel<<<grid, 256, 0, stream>>>(rel.buckets, static_cast<const uint8_t*>(rel.table), rel.stride_bucket, rel.stride_head,
-                                   rel.table_f32, rel.bias.zero, rel.bias.width, const_cast<float*>(rel.bias.values),
+                                   rel.table_f32, rel.bias.zero, rel.bias.width, rel.bias.stride, const_cast<float*>(rel.bias.values),
                                    const_cast<int*>(rel.bias.bucket_of));
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   FO_CUDA_CHECK(cudaGetLastError());
@@ -306,7 +309,7 @@ extern "C" int fo_rel_attn_fwd(const void* q, const void* k, const void* v, void
   RelArgs rel;
   if (int rc = make_rel_args(&rel, Sq, Sk, table, table_dtype, table_strides, starts, n_starts, two_sided, query_offset, dtype))
     return rc;
-  FO_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0, "workspace must be given, 4-byte aligned");
+  FO_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be given, 16-byte aligned");
   FO_REQUIRE(H > 0, "H must be positive (got %d)", H);
   if (int rc = check_bias_strides(bias, bias_strides)) return rc;
   fo::AttnExtras ex;
@@ -333,7 +336,7 @@ extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, cons
   // the table itself is not read again: its expanded form is
   if (int rc = make_rel_args(&rel, Sq, Sk, workspace, table_dtype, no_strides, starts, n_starts, two_sided, query_offset, dtype))
     return rc;
-  FO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 3) == 0, "workspace must be 4-byte aligned");
+  FO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be 16-byte aligned");
   FO_REQUIRE(H > 0 && B > 0, "B and H must be positive (got %d %d)", B, H);
   FO_REQUIRE(dtable == nullptr || partials != nullptr, "the table's gradient needs its workspace");
   FO_REQUIRE((reinterpret_cast<uintptr_t>(partials) & 7) == 0, "partials must be 8-byte aligned");

@@ -225,21 +225,24 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const uint32_t drop_row = prm.ex.drop_base +
                               static_cast<uint32_t>(bh) * static_cast<uint32_t>(prm.Sq) * static_cast<uint32_t>(prm.Sk) +
                               static_cast<uint32_t>(row) * static_cast<uint32_t>(prm.Sk);
-    // the scores are scaled when the bias is added, not in the exponent
-    const float exp_scale = 1.f;
+    // The scores are scaled when the bias is added, not in the exponent; but away from the diagonal a
+    // relative bias is a constant, and without a vector bias beside it nothing is added to the scores
+    // there: they are scaled in the exponent, and the constant joins the reference maximum.
+    float exp_scale = 1.f, exp_add = 0.f;
     // a row-independent bias goes through shared memory, fetched one 128-key tile ahead
     const uint8_t* bias_vec = nullptr;
     float* sb = s_bias + s * 256;
     float bias_next = 0.f;
     // a relative bias: this row's values by key (read only near the diagonal), and the two far constants
-    const float* rel_row = nullptr;
+    const float4* rel_row = nullptr;
     float rel_left = 0.f, rel_right = 0.f;
     const int warp_row = q0 + (warp & 3) * 32 + q_off;  // key position of the warp's first row
     if constexpr (rel_bias) {
-      rel_row = prm.rel.values + static_cast<int64_t>(h) * prm.rel.width;
-      rel_left = __ldg(rel_row);
-      rel_right = __ldg(rel_row + prm.rel.width - 1);
-      rel_row += static_cast<int64_t>(prm.rel.zero) - row - q_off;
+      rel_left = rel_value(prm.rel, h, -prm.rel.zero);
+      rel_right = rel_value(prm.rel, h, prm.rel.width);
+      // value of key 0, which may lie before the vector; those read do not
+      const int x = prm.rel.zero - row - q_off, s4 = x & 3;
+      rel_row = rel_vector(prm.rel, h, s4) + ((x - s4) >> 2);
     }
     auto load_vec = [&](int col) {
       if constexpr (rel_bias) return scaled_or_masked(load_elem<kBf16>(bias_vec, col, prm.ex.bias_f32));
@@ -311,32 +314,39 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       const bool need_mask = (k0n + kStepN > prm.Sk) || (prm.causal && k0n + kStepN - 1 > q0 + q_off);
       // relative positions of the warp's 32 rows and the step's keys: d_last - 94 to d_last
       const int d_last = k0n + kStepN - 1 - warp_row;
-      const bool rel_near = rel_bias && d_last > -prm.rel.far_left && d_last - (kStepN + 30) < prm.rel.far_right;
-      const float rel_far = d_last > -prm.rel.far_left ? rel_right : rel_left;
+      const RelSide side = rel_bias ? rel_side(prm.rel, d_last - (kStepN + 30), d_last) : kRelNear;
+      if constexpr (rel_bias) {
+        exp_add = side == kRelLeft ? rel_left : side == kRelRight ? rel_right : 0.f;
+        exp_scale = vec_bias || side == kRelNear ? 1.f : prm.scale_log2;
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         tmem_ld_wait(sr[c]);
         if ((warp & 3) == 0 && tn > 0) trace_event(prm, s, tn - 1, c == 0 ? 1 : 4);  // loads in
         if constexpr (rel_bias) {
           const float4* bv = reinterpret_cast<const float4*>(sb + ((tn >> 1) & 1) * 128 + ((tn & 1) ^ first) * kStepN + c * 32);
-          if (rel_near) {
-            float bb[32];
+          if (side == kRelNear) {
+            const float4* const rv = rel_row + (k0n >> 2) + c * 8;
+            float4 r4[8];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) bb[i] = __ldg(rel_row + k0n + c * 32 + i);
+            for (int i = 0; i < 8; ++i) r4[i] = __ldg(rv + i);
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              float4 v4 = make_float4(0.f, 0.f, 0.f, 0.f);
-              if constexpr (vec_bias) v4 = bv[i >> 2];
-              add_bias2(c, i, make_float2(bb[i] + v4.x, bb[i + 1] + v4.y));
-              add_bias2(c, i + 2, make_float2(bb[i + 2] + v4.z, bb[i + 3] + v4.w));
+              float2 lo = make_float2(r4[i >> 2].x, r4[i >> 2].y), hi = make_float2(r4[i >> 2].z, r4[i >> 2].w);
+              if constexpr (vec_bias) {
+                const float4 v4 = bv[i >> 2];
+                lo = __fadd2_rn(lo, make_float2(v4.x, v4.y));
+                hi = __fadd2_rn(hi, make_float2(v4.z, v4.w));
+              }
+              add_bias2(c, i, lo);
+              add_bias2(c, i + 2, hi);
             }
-          } else {
+          } else if constexpr (vec_bias) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              float4 v4 = make_float4(0.f, 0.f, 0.f, 0.f);
-              if constexpr (vec_bias) v4 = bv[i >> 2];
-              add_bias2(c, i, make_float2(rel_far + v4.x, rel_far + v4.y));
-              add_bias2(c, i + 2, make_float2(rel_far + v4.z, rel_far + v4.w));
+              const float4 v4 = bv[i >> 2];
+              add_bias2(c, i, make_float2(v4.x, v4.y));
+              add_bias2(c, i + 2, make_float2(v4.z, v4.w));
             }
           }
         } else if constexpr (vec_bias) {
@@ -403,7 +413,7 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     issue_load(first, 0);
     issue_load(first, 1);
     prep_loads(first);
-    m_run = row_max() * exp_scale;
+    m_run = rel_bias ? fmaf(row_max(), exp_scale, exp_add) : row_max() * exp_scale;
 
     // The exponentials of a step do not wait for the step's own row maximum: they are taken
     // against the reference maximum the row already has (lazy rescaling moves it only when the
@@ -419,6 +429,7 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       const uint32_t drop_idx = drop_row + (kTight ? static_cast<uint32_t>(k0) : 0u);
       const uint32_t tS = tS_tile + u * kStepN;
       float neg_m = (m_run == -INFINITY) ? 0.f : -m_run;
+      if constexpr (rel_bias) neg_m += exp_add;
       if (ping_pong) named_barrier_sync_dep(s ? kTurn1 : kTurn0, kTurnCount, neg_m);  // exponentials start after this
       if ((warp & 3) == 0) trace_event(prm, s, t, 0);  // turn taken
       const float2 sc2 = make_float2(exp_scale, exp_scale);
@@ -470,7 +481,8 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       };
       exp_pass(neg_m, true);
       // did a row outgrow its reference?
-      const float m_cand = fmaxf(m_run, fmaxf(mxa, mxb) * exp_scale);
+      const float mx = fmaxf(mxa, mxb);
+      const float m_cand = fmaxf(m_run, rel_bias ? fmaf(mx, exp_scale, exp_add) : mx * exp_scale);
       const bool grow = m_cand - m_run > kRescaleThreshold;  // false when both are -inf (NaN)
       float alpha = 1.f;
       if (__any_sync(0xffffffffu, grow)) {
@@ -479,7 +491,7 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
         alpha = grow ? fast_exp2(m_run - m_use) : 1.f;
         m_run = m_new;
-        exp_pass(-m_use, false);
+        exp_pass(rel_bias ? exp_add - m_use : -m_use, false);
       }
       // hand the rescale factor to the correction warps
       alpha_slot[u * 128] = alpha;

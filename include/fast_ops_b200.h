@@ -158,7 +158,7 @@ int fo_flash_attn_bwd_ex(const void* q, const void* k, const void* v, const void
  *   table      : device pointer, fp32 or the dtype of q (table_dtype), element (bucket, head) at
  *                table + bucket*s[0] + head*s[1] with s = table_strides in elements (non-negative).
  *   query_offset : key position of query row 0, in [0, 2^29].
- *   workspace  : device memory of fo_rel_attn_workspace(...) bytes, 4-byte aligned.  The forward writes
+ *   workspace  : device memory of fo_rel_attn_workspace(...) bytes, 16-byte aligned.  The forward writes
  *                the expanded bias there; the backward must be given it as the forward left it.
  *   bias       : as in fo_flash_attn_fwd_ex, but the same for every query row: bias_strides[2] = 0.
  *                Entries of -1e6 and below mask like -inf, in the table too.
