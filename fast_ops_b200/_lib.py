@@ -46,7 +46,7 @@ SIGNATURES = {
                               _PTR, _I64P, _c.c_int, _c.c_float, _c.c_uint64, _c.c_uint64,
                               _c.c_int, _PTR]),
     "fo_rel_attn_workspace": (_c.c_int64, [_c.c_int, _c.c_int, _c.c_int, _c.POINTER(_c.c_int), _c.c_int, _c.c_int,
-                                           _c.c_int]),
+                                           _c.c_int, _c.c_int64]),
     "fo_rel_attn_bwd_workspace": (_c.c_int64, [_c.c_int] * 7),
     "fo_rel_attn_fwd": (_c.c_int, [_PTR] * 5 + [_c.c_int] * 5 + [_I64P] * 4 + [_c.c_int, _c.c_int, _c.c_float] +
                         [_PTR, _I64P, _c.c_int, _c.POINTER(_c.c_int), _c.c_int, _c.c_int, _c.c_int, _PTR,

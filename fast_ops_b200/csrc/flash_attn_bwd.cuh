@@ -258,7 +258,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   constexpr bool rel_bias = (kExt & kBwdRelBias) != 0;
   const int q_off = rel_bias ? prm.rel.offset : 0;  // query row i stands at key position i + q_off
   const int i0 = prm.causal ? min(rel_bias ? max(k0 - q_off, 0) / kBlockM : j, n_q_tiles) : 0;
-  const int n_iter = n_q_tiles - i0;
+  // (none if all the tile's keys are masked by a vector bias beside a relative one)
+  const int n_iter = rel_bias && k0 >= rel_keys(prm.rel, b, h, prm.Sk) ? 0 : n_q_tiles - i0;
   int* const dstat = prm.device_status;
 
   if (tid == 0) {
@@ -358,9 +359,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // values of query rows 3 to 0, which may lie behind the vector; those read do not
       const int x = prm.rel.zero + key - q_off - 3, s4 = x & 3;
       rel_col = rel_vector(prm.rel, h, s4) + ((x - s4) >> 2);
-      if (prm.ex.bias != nullptr && key_ok)
-        bias_key = scaled_or_masked(load_elem<kBf16>(static_cast<const uint8_t*>(prm.ex.bias),
-                                                     b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h + key, prm.ex.bias_f32));
+      if (prm.rel.vec != nullptr) bias_key = __ldg(prm.rel.vec + rel_vec_row(prm.rel, b, h) * prm.rel.vec_width + key);
       if (prm.rel.acc != nullptr) {
         rel_acc = prm.rel.acc + ((static_cast<int64_t>(bh) * gridDim.x + j) * kCW + warp) * prm.rel.num_buckets;
         for (int x = lane; x < prm.rel.num_buckets; x += 32) rel_acc[x] = 0.f;

@@ -307,7 +307,7 @@ int fo::attn_fwd_impl(const void* q, const void* k, const void* v, void* o, floa
     if (int rc = fo::check_layout(k, B, Hkv, Sk, D, k_strides, "k", ks)) return rc;
     if (int rc = fo::check_layout(v, B, Hkv, Sk, D, v_strides, "v", vs)) return rc;
     if (rel && lse != nullptr)  // a backward may follow, whose tile kernels read the expanded bias
-      if (int rc = fo::launch_rel_expand(*rel, H, dtype == FO_BF16, static_cast<cudaStream_t>(stream))) return rc;
+      if (int rc = fo::launch_rel_expand(*rel, *ex, H, Sk, dtype == FO_BF16, static_cast<cudaStream_t>(stream))) return rc;
     return decode(q, k, v, o, lse, B, H, rel ? keys : Sk, D, qs, ks, vs, o_strides, kv_bcast, dtype, softmax_scale, status,
                   rel, ex, info->num_sms, device, static_cast<cudaStream_t>(stream));
   }
@@ -359,8 +359,16 @@ int fo::attn_fwd_impl(const void* q, const void* k, const void* v, void* o, floa
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == FO_BF16;
   if (rel) {
-    if (int rc = fo::launch_rel_expand(*rel, H, bf16, s)) return rc;
-    return fo::launch_fwd_rel(tq, tk, tv, prm, bf16, s);
+    if (int rc = fo::launch_rel_expand(*rel, *ex, H, Sk, bf16, s)) return rc;
+    const int64_t pair_items = static_cast<int64_t>((prm.num_q_tiles + 1) / 2) * B * H;
+    const int room = Dk == 64 ? fo::Ws64sConfig<64>::kMaxRelStride : fo::Ws64sConfig<128>::kMaxRelStride;
+    const bool half_tiles = !ex->dropout && prm.rel.stride <= room &&
+                            (impl == AttnImpl::kShort64 || (impl == AttnImpl::kAuto && (Dk == 64 || Sk <= 1024 || pair_items <= info->num_sms)));
+    if (half_tiles) {
+      if (int rc = make_tensor_map(&tk, k, dtype, B, Hkv, Sk, D, k_strides, "k", fo::kStepN)) return rc;
+      if (int rc = make_tensor_map(&tv, v, dtype, B, Hkv, Sk, D, v_strides, "v", fo::kStepN)) return rc;
+    }
+    return fo::launch_fwd_rel(tq, tk, tv, prm, half_tiles, bf16, s);
   }
   if (impl == AttnImpl::kAuto) {
     // The 64-key-step kernel is the faster one at every shape measured (same box, hot loop, bf16

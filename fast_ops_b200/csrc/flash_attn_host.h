@@ -19,6 +19,8 @@ struct RelArgs {
   int64_t stride_bucket, stride_head;  // elements
   int table_f32;                       // 1: fp32, 0: the 16-bit type of q
   RelBias bias;                        // what the tile kernels read
+  int64_t bias_rows;                   // rows of the expanded vector bias, of bias_heads heads each
+  int bias_heads;
 };
 
 // The forward and the backward behind all entry points (flash_attn_fwd.cu, flash_attn_bwd.cu).
@@ -38,12 +40,13 @@ int attn_bwd_impl(const void* q, const void* k, const void* v, const void* o, co
                   int device, void* stream);
 
 // The launches of the kernels built for a relative bias (flash_attn_rel.cu), called by the two above.
-// The bias vector is expanded by launch_rel_expand before the first of them.
-int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& prm, bool bf16,
-                   cudaStream_t stream);
+// The bias is brought into the form they read by launch_rel_expand before the first of them.  `half_tiles`:
+// tk and tv have boxes of 64 keys, for the kernel with one query tile per CTA.
+int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& prm, bool half_tiles,
+                   bool bf16, cudaStream_t stream);
 int launch_bwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                    const CUtensorMap& tdq, const AttnBwdParams& prm, bool bf16, cudaStream_t stream);
-int launch_rel_expand(const RelArgs& rel, int H, bool bf16, cudaStream_t stream);
+int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, bool bf16, cudaStream_t stream);
 
 struct DecodeParams;
 int launch_decode_rel(const DecodeParams& prm, const RelArgs& rel, const AttnExtras& ex, int B, int H, int Sk, int D,

@@ -9,6 +9,7 @@
 #include "flash_attn_decode.cuh"
 #include "flash_attn_host.h"
 #include "flash_attn_ws64r.cuh"
+#include "flash_attn_ws64s.cuh"
 #include "fo_host.h"
 
 namespace {
@@ -17,21 +18,74 @@ using fo::RelArgs;
 using fo::RelBias;
 using fo::RelBuckets;
 
-// values[h][s][x] = log2(e) * table[bucket(x + s - zero)][h], and the buckets themselves.
+// The bias in the form the tile kernels read: values[h][s][x] = log2(e) * table[bucket(x + s - zero)][h], the
+// buckets themselves, and the rows of a vector bias.  The first blocks make the former, 256 positions of one
+// head each; then one block takes each row.
+struct ExpandParams {
+  RelBuckets buckets;
+  const uint8_t* table;
+  int64_t stride_bucket, stride_head;
+  int table_f32;
+  const uint8_t* bias;  // vector bias as the caller gave it, or null
+  int64_t bias_stride_b, bias_stride_h;
+  int bias_f32;
+  int bias_heads;       // heads of the rows made of it
+  int H, Sk, zero, width, stride, value_blocks, vec_width;
+  float* values;
+  int* bucket_of;
+  float* vec;
+  int4* vec_extent;
+};
+
 template <bool kBf16>
 __global__ void __launch_bounds__(256)
-rel_expand_kernel(const __grid_constant__ RelBuckets buckets, const uint8_t* __restrict__ table, int64_t stride_bucket,
-                  int64_t stride_head, int table_f32, int zero, int width, int stride, float* __restrict__ values,
-                  int* __restrict__ bucket_of) {
-  const int x = blockIdx.x * 256 + threadIdx.x;
-  const int h = blockIdx.y;
-  if (x >= width) return;
-  const int bucket = fo::rel_bucket(buckets, x - zero);
-  const float v = fo::scaled_or_masked(fo::load_elem<kBf16>(table, bucket * stride_bucket + h * stride_head, table_f32));
+rel_expand_kernel(const __grid_constant__ ExpandParams prm) {
+  const int per_head = (prm.width + 255) / 256;
+  if (static_cast<int>(blockIdx.x) < prm.value_blocks) {
+    const int h = blockIdx.x / per_head;
+    const int x = (blockIdx.x - h * per_head) * 256 + threadIdx.x;
+    if (x >= prm.width) return;
+    const int bucket = fo::rel_bucket(prm.buckets, x - prm.zero);
+    const float v = fo::scaled_or_masked(
+        fo::load_elem<kBf16>(prm.table, bucket * prm.stride_bucket + h * prm.stride_head, prm.table_f32));
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
-    if (x >= s) values[(static_cast<int64_t>(h) * 4 + s) * stride + x - s] = v;
-  if (h == 0) bucket_of[x] = bucket;
+    for (int s = 0; s < 4; ++s)
+      if (x >= s) prm.values[(static_cast<int64_t>(h) * 4 + s) * prm.stride + x - s] = v;
+    if (h == 0) prm.bucket_of[x] = bucket;
+    return;
+  }
+  const int row = blockIdx.x - prm.value_blocks;
+  const int b = row / prm.bias_heads, h = row - b * prm.bias_heads;
+  const int64_t src = b * prm.bias_stride_b + h * prm.bias_stride_h;
+  float* const dst = prm.vec + static_cast<int64_t>(row) * prm.vec_width;
+  int end = 0, first = prm.vec_width, last = -1;
+#pragma unroll 4
+  for (int key = threadIdx.x; key < prm.vec_width; key += 256) {
+    const float v = key < prm.Sk ? fo::scaled_or_masked(fo::load_elem<kBf16>(prm.bias, src + key, prm.bias_f32)) : 0.f;
+    dst[key] = v;
+    if (v != 0.f) {
+      first = min(first, key);
+      last = key;
+    }
+    if (key < prm.Sk && !(v == __int_as_float(0xff800000))) end = key + 1;
+  }
+  first = __reduce_min_sync(0xffffffffu, first);
+  last = __reduce_max_sync(0xffffffffu, last);
+  end = __reduce_max_sync(0xffffffffu, end);
+  __shared__ int found[8][3];
+  if ((threadIdx.x & 31) == 0) {
+    found[threadIdx.x >> 5][0] = first;
+    found[threadIdx.x >> 5][1] = last;
+    found[threadIdx.x >> 5][2] = end;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < 8; ++w) {
+    first = min(first, found[w][0]);
+    last = max(last, found[w][1]);
+    end = max(end, found[w][2]);
+  }
+  prm.vec_extent[row] = make_int4(end, first / 64, last < 0 ? 0 : last / 64 + 1, 0);
 }
 
 template <class T>
@@ -69,7 +123,8 @@ rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, i
     const float2* const row = rel.tile_sums + (bh * n_q_tiles + i) * n_k_tiles * warps + p * 4;
     const int q_first = i * fo::kBlockM + p * cols + rel.offset;  // key position of the part's first query
     // key tiles that this query tile sees (the backward visits no others)
-    int n = n_k_tiles;
+    const int b = static_cast<int>(bi / n_q_tiles);
+    int n = rel.vec == nullptr ? n_k_tiles : (fo::rel_keys(rel, b, h, n_k_tiles * fo::kBlockN) + fo::kBlockN - 1) / fo::kBlockN;
     if (causal) n = min(n, (i * fo::kBlockM + fo::kBlockM - 1 + rel.offset) / fo::kBlockN + 1);
     double ds = 0, mass = 0, ds_side[2] = {0, 0}, mass_side[2] = {0, 0};
     for (int x = lane; x < n * 4; x += 32) {
@@ -132,7 +187,7 @@ rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, i
 
 // Checks of the relative bias's own arguments; fills everything of `rel` but the device pointers of the
 // expanded vector.
-int make_rel_args(RelArgs* rel, int Sq, int Sk, const void* table, int table_dtype, const int64_t* table_strides,
+int make_rel_args(RelArgs* rel, int H, int Sq, int Sk, const void* table, int table_dtype, const int64_t* table_strides,
                   const int* starts, int n_starts, int two_sided, int query_offset, int dtype) {
   FO_REQUIRE(dtype == FO_F16 || dtype == FO_BF16, "attention inputs must be fp16 or bf16 (got dtype %d)", dtype);
   FO_REQUIRE(table && table_strides && starts, "null relative bias argument");
@@ -162,15 +217,36 @@ int make_rel_args(RelArgs* rel, int Sq, int Sk, const void* table, int table_dty
   bias.far_right = two_sided ? std::min(std::max(last, 1), Sk) : 0;
   bias.zero = bias.far_left + fo::kRelMargin;
   bias.width = bias.zero + bias.far_right + fo::kRelMargin + 1;
-  bias.stride = (bias.width + 3) / 4 * 4;
+  bias.stride = (bias.width - 8 + 31) / 32 * 32 + 8;
+  FO_REQUIRE(H <= 0 || 4LL * H * bias.stride < (1LL << 31), "too many heads for bucket starts up to %d", last);
   return FO_OK;
 }
 
-int64_t expanded_bytes(const RelBias& bias, int H) { return (static_cast<int64_t>(H) * 4 + 1) * bias.stride * 4; }
+// The expanded bias in a workspace: values, rows of the vector bias, buckets.
+int64_t expanded_bytes(const RelBias& bias, int H, int64_t bias_rows, int Sk) {
+  const int64_t width = fo::rel_vec_width(Sk);
+  return (static_cast<int64_t>(H) * 4 * bias.stride + bias_rows * width + bias.stride) * 4 + bias_rows * 16;
+}
 
-void set_expanded(RelBias* bias, void* workspace, int H) {
-  bias->values = static_cast<const float*>(workspace);
-  bias->bucket_of = reinterpret_cast<const int*>(bias->values + static_cast<int64_t>(H) * 4 * bias->stride);
+int set_expanded(RelArgs* rel, void* workspace, const fo::AttnExtras& ex, int B, int H, int Sk) {
+  FO_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be given, 16-byte aligned");
+  FO_REQUIRE(B > 0 && H > 0, "B and H must be positive (got %d %d)", B, H);
+  RelBias& bias = rel->bias;
+  bias.values = static_cast<const float*>(workspace);
+  const float* next = bias.values + static_cast<int64_t>(H) * 4 * bias.stride;
+  if (ex.bias != nullptr) {
+    // one row for each batch and head that has its own; where the caller's bias is broadcast, the row is too
+    rel->bias_heads = ex.bias_stride_h != 0 ? H : 1;
+    rel->bias_rows = static_cast<int64_t>(ex.bias_stride_b != 0 ? B : 1) * rel->bias_heads;
+    bias.vec_width = fo::rel_vec_width(Sk);
+    bias.vec = next;
+    bias.vec_row_b = ex.bias_stride_b != 0 ? rel->bias_heads : 0;
+    bias.vec_row_h = ex.bias_stride_h != 0 ? 1 : 0;
+    next += rel->bias_rows * bias.vec_width;
+  }
+  bias.bucket_of = reinterpret_cast<const int*>(next);
+  bias.vec_extent = reinterpret_cast<const int4*>(bias.bucket_of + bias.stride);  // every part is a multiple of 16 bytes
+  return FO_OK;
 }
 
 // Warps of the backward that sum for the table's gradient, per key tile.
@@ -201,32 +277,55 @@ int check_bias_strides(const void* bias, const int64_t* strides) {
 
 namespace fo {
 
-int launch_rel_expand(const RelArgs& rel, int H, bool bf16, cudaStream_t stream) {
-  const dim3 grid((rel.bias.width + 255) / 256, H);
+int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, bool bf16, cudaStream_t stream) {
+  ExpandParams prm;
+  prm.buckets = rel.buckets;
+  prm.table = static_cast<const uint8_t*>(rel.table);
+  prm.stride_bucket = rel.stride_bucket;
+  prm.stride_head = rel.stride_head;
+  prm.table_f32 = rel.table_f32;
+  prm.bias = static_cast<const uint8_t*>(ex.bias);
+  prm.bias_stride_b = ex.bias_stride_b;
+  prm.bias_stride_h = ex.bias_stride_h;
+  prm.bias_f32 = ex.bias_f32;
+  prm.bias_heads = rel.bias_heads;
+  prm.H = H;
+  prm.Sk = Sk;
+  prm.zero = rel.bias.zero;
+  prm.width = rel.bias.width;
+  prm.stride = rel.bias.stride;
+  prm.vec_width = rel_vec_width(Sk);
+  prm.values = const_cast<float*>(rel.bias.values);
+  prm.bucket_of = const_cast<int*>(rel.bias.bucket_of);
+  prm.vec = const_cast<float*>(rel.bias.vec);
+  prm.vec_extent = const_cast<int4*>(rel.bias.vec_extent);
+  const int64_t value_blocks = static_cast<int64_t>((prm.width + 255) / 256) * H;
+  const int64_t blocks = value_blocks + rel.bias_rows;
+  FO_REQUIRE(blocks <= 0x7fffffff, "the bias is too large for one launch");
+  prm.value_blocks = static_cast<int>(value_blocks);
   auto kernel = bf16 ? rel_expand_kernel<true> : rel_expand_kernel<false>;
-  kernel<<<grid, 256, 0, stream>>>(rel.buckets, static_cast<const uint8_t*>(rel.table), rel.stride_bucket, rel.stride_head,
-                                   rel.table_f32, rel.bias.zero, rel.bias.width, rel.bias.stride, const_cast<float*>(rel.bias.values),
-                                   const_cast<int*>(rel.bias.bucket_of));
+  kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(prm);
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   FO_CUDA_CHECK(cudaGetLastError());
   return FO_OK;
 }
 
-int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& prm, bool bf16,
-                   cudaStream_t stream) {
-  const int form = kFwdRelBias | (prm.ex.bias != nullptr ? kFwdVecBias : 0) | (prm.ex.dropout ? kFwdDropout : 0);
-#define FO_REL_FORM(M)                                                                                                \
-  if (form == (M)) {                                                                                                  \
-    if (prm.d_real > 64)                                                                                              \
-      return bf16 ? launch_ws64r<128, true, (M)>(tq, tk, tv, prm, stream) : launch_ws64r<128, false, (M)>(tq, tk, tv, prm, stream); \
-    return bf16 ? launch_ws64r<64, true, (M)>(tq, tk, tv, prm, stream) : launch_ws64r<64, false, (M)>(tq, tk, tv, prm, stream);     \
+int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const AttnParams& prm, bool half_tiles,
+                   bool bf16, cudaStream_t stream) {
+#define FO_REL_FORM(LAUNCH, DK, ...) \
+  bf16 ? LAUNCH<DK, true, __VA_ARGS__>(tq, tk, tv, prm, stream) : LAUNCH<DK, false, __VA_ARGS__>(tq, tk, tv, prm, stream)
+  const bool wide = prm.d_real > 64, vec = prm.rel.vec != nullptr;
+  if (half_tiles) {
+    if (wide) return vec ? FO_REL_FORM(launch_ws64s, 128, 128, (kFwdRelBias | kFwdVecBias)) : FO_REL_FORM(launch_ws64s, 128, 128, kFwdRelBias);
+    return vec ? FO_REL_FORM(launch_ws64s, 64, 64, (kFwdRelBias | kFwdVecBias)) : FO_REL_FORM(launch_ws64s, 64, 64, kFwdRelBias);
   }
-  FO_REL_FORM(kFwdRelBias)
-  FO_REL_FORM(kFwdRelBias | kFwdVecBias)
-  FO_REL_FORM(kFwdRelBias | kFwdDropout)
-  FO_REL_FORM(kFwdRelBias | kFwdVecBias | kFwdDropout)
+  if (prm.ex.dropout) {
+    if (wide) return vec ? FO_REL_FORM(launch_ws64r, 128, (kFwdRelBias | kFwdVecBias | kFwdDropout)) : FO_REL_FORM(launch_ws64r, 128, (kFwdRelBias | kFwdDropout));
+    return vec ? FO_REL_FORM(launch_ws64r, 64, (kFwdRelBias | kFwdVecBias | kFwdDropout)) : FO_REL_FORM(launch_ws64r, 64, (kFwdRelBias | kFwdDropout));
+  }
+  if (wide) return vec ? FO_REL_FORM(launch_ws64r, 128, (kFwdRelBias | kFwdVecBias)) : FO_REL_FORM(launch_ws64r, 128, kFwdRelBias);
+  return vec ? FO_REL_FORM(launch_ws64r, 64, (kFwdRelBias | kFwdVecBias)) : FO_REL_FORM(launch_ws64r, 64, kFwdRelBias);
 #undef FO_REL_FORM
-  return fail(FO_ERR_UNSUPPORTED, "no kernel of this form");
 }
 
 int launch_bwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
@@ -273,17 +372,17 @@ int launch_decode_rel(const DecodeParams& prm, const RelArgs& args, const AttnEx
 }  // namespace fo
 
 extern "C" int64_t fo_rel_attn_workspace(int H, int Sq, int Sk, const int* starts, int n_starts, int two_sided,
-                                         int query_offset) {
+                                         int query_offset, int64_t bias_rows) {
   fo::clear_error();
   RelArgs rel;
   const int64_t strides[2] = {0, 0};
   const float table = 0;
-  if (make_rel_args(&rel, Sq, Sk, &table, FO_F32, strides, starts, n_starts, two_sided, query_offset, FO_BF16)) return -1;
-  if (H <= 0) {
-    fo::fail(FO_ERR_INVALID_ARGUMENT, "H must be positive (got %d)", H);
+  if (make_rel_args(&rel, H, Sq, Sk, &table, FO_F32, strides, starts, n_starts, two_sided, query_offset, FO_BF16)) return -1;
+  if (H <= 0 || bias_rows < 0) {
+    fo::fail(FO_ERR_INVALID_ARGUMENT, "H must be positive and bias_rows not negative (got %d %lld)", H, (long long)bias_rows);
     return -1;
   }
-  return expanded_bytes(rel.bias, H);
+  return expanded_bytes(rel.bias, H, bias_rows, Sk);
 }
 
 extern "C" int64_t fo_rel_attn_bwd_workspace(int B, int H, int Sq, int Sk, int D, int num_buckets, int dropout) {
@@ -307,14 +406,12 @@ extern "C" int fo_rel_attn_fwd(const void* q, const void* k, const void* v, void
                                int device, void* stream) {
   fo::clear_error();
   RelArgs rel;
-  if (int rc = make_rel_args(&rel, Sq, Sk, table, table_dtype, table_strides, starts, n_starts, two_sided, query_offset, dtype))
+  if (int rc = make_rel_args(&rel, H, Sq, Sk, table, table_dtype, table_strides, starts, n_starts, two_sided, query_offset, dtype))
     return rc;
-  FO_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be given, 16-byte aligned");
-  FO_REQUIRE(H > 0, "H must be positive (got %d)", H);
   if (int rc = check_bias_strides(bias, bias_strides)) return rc;
   fo::AttnExtras ex;
   if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset)) return rc;
-  set_expanded(&rel.bias, workspace, H);
+  if (int rc = set_expanded(&rel, workspace, ex, B, H, Sk)) return rc;
   return fo::attn_fwd_impl(q, k, v, o, lse, B, H, Sq, Sk, D, q_strides, k_strides, v_strides, o_strides, dtype, causal,
                            softmax_scale, &ex, &rel, device, stream);
 }
@@ -334,17 +431,15 @@ extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, cons
   RelArgs rel;
   const int64_t no_strides[2] = {0, 0};
   // the table itself is not read again: its expanded form is
-  if (int rc = make_rel_args(&rel, Sq, Sk, workspace, table_dtype, no_strides, starts, n_starts, two_sided, query_offset, dtype))
+  if (int rc = make_rel_args(&rel, H, Sq, Sk, workspace, table_dtype, no_strides, starts, n_starts, two_sided, query_offset, dtype))
     return rc;
-  FO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be 16-byte aligned");
-  FO_REQUIRE(H > 0 && B > 0, "B and H must be positive (got %d %d)", B, H);
   FO_REQUIRE(dtable == nullptr || partials != nullptr, "the table's gradient needs its workspace");
   FO_REQUIRE((reinterpret_cast<uintptr_t>(partials) & 7) == 0, "partials must be 8-byte aligned");
   FO_REQUIRE(reinterpret_cast<uintptr_t>(dtable) % (table_dtype == FO_F32 ? 4 : 2) == 0, "dtable is not aligned to its elements");
   if (int rc = check_bias_strides(bias, bias_strides)) return rc;
   fo::AttnExtras ex;
   if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset)) return rc;
-  set_expanded(&rel.bias, const_cast<void*>(workspace), H);
+  if (int rc = set_expanded(&rel, const_cast<void*>(workspace), ex, B, H, Sk)) return rc;
   if (dtable != nullptr) {
     rel.bias.tile_sums = reinterpret_cast<float2*>(partials);
     rel.bias.acc = partials + tile_sum_floats(B, H, Sq, Sk, D, ex.dropout != 0);

@@ -92,8 +92,9 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   // keys visible to query tile 0 / 1 of this pair, in 64-key steps (T) and 128-key tiles (n)
   constexpr bool rel_bias = (kExt & kFwdRelBias) != 0;
   const int q_off = rel_bias ? prm.rel.offset : 0;  // query row i stands at key position i + q_off
-  const int vis0 = prm.causal ? min(prm.Sk, (2 * pair + 1) * kBlockM + q_off) : prm.Sk;
-  const int vis1 = prm.causal ? min(prm.Sk, (2 * pair + 2) * kBlockM + q_off) : prm.Sk;
+  const int keys = rel_bias ? rel_keys(prm.rel, b, h, prm.Sk) : prm.Sk;
+  const int vis0 = prm.causal ? min(keys, (2 * pair + 1) * kBlockM + q_off) : keys;
+  const int vis1 = prm.causal ? min(keys, (2 * pair + 2) * kBlockM + q_off) : keys;
   const int n0 = (vis0 + kBlockN - 1) / kBlockN;
   const int n1 = (vis1 + kBlockN - 1) / kBlockN;
   const int T0 = 2 * n0, T1 = 2 * n1;  // T1 >= T0 >= 2
@@ -111,7 +112,7 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     float bias_first = 0.f, bias_last = 0.f;
     if (n1 > 1) {
       const int64_t row = min((2 * pair + 1) * kBlockM, prm.Sq - 1);
-      if constexpr ((kExt & ~(kFwdRelBias | kFwdDropout)) != 0) {
+      if constexpr (!rel_bias) {
         const uint8_t* const p = static_cast<const uint8_t*>(prm.ex.bias) +
                                  (b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h + row * prm.ex.bias_stride_q) *
                                      (prm.ex.bias_f32 ? 4 : 2);
@@ -120,8 +121,13 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       }
       if constexpr (rel_bias) {
         const int d0 = -static_cast<int>(row) - q_off;  // relative position of key 0
-        bias_first += rel_value(prm.rel, h, d0);
-        bias_last += rel_value(prm.rel, h, d0 + vis0 - 1);
+        bias_first = rel_value(prm.rel, h, d0);
+        bias_last = rel_value(prm.rel, h, d0 + vis0 - 1);
+        if (prm.rel.vec != nullptr) {
+          const float* const v = prm.rel.vec + rel_vec_row(prm.rel, b, h) * prm.rel.vec_width;
+          bias_first += __ldg(v);
+          bias_last += __ldg(v + vis0 - 1);
+        }
       }
     }
     const int status = *reinterpret_cast<volatile int*>(prm.device_status);
@@ -214,7 +220,8 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const uint32_t tS_tile = tmem_base + Cfg::kColS0 + s * kBlockN + lane_base;
     float* alpha_slot = s_alpha + s * 256 + r;
     float m_run = -INFINITY, l_run = 0.f;
-    constexpr bool vec_bias = (kExt & kFwdVecBias) != 0, mat_bias16 = (kExt & kFwdMatBias) != 0;
+    constexpr bool rel_vec = rel_bias && (kExt & kFwdVecBias) != 0;  // a vector bias beside a relative one
+    constexpr bool vec_bias = !rel_bias && (kExt & kFwdVecBias) != 0, mat_bias16 = (kExt & kFwdMatBias) != 0;
     constexpr bool mat_bias = mat_bias16 || (kExt & kFwdMatBias32) != 0;
     constexpr bool has_drop = (kExt & kFwdDropout) != 0;
     const uint8_t* bias_row = nullptr;
@@ -235,6 +242,8 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     float bias_next = 0.f;
     // a relative bias: this row's values by key (read only near the diagonal), and the two far constants
     const float4* rel_row = nullptr;
+    const float* rel_vec_keys = nullptr;  // this head's row of the vector bias,
+    int vec_first = 0, vec_last = 0;      // and the keys between which it is not zero (whole steps)
     float rel_left = 0.f, rel_right = 0.f;
     const int warp_row = q0 + (warp & 3) * 32 + q_off;  // key position of the warp's first row
     if constexpr (rel_bias) {
@@ -243,16 +252,20 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       // value of key 0, which may lie before the vector; those read do not
       const int x = prm.rel.zero - row - q_off, s4 = x & 3;
       rel_row = rel_vector(prm.rel, h, s4) + ((x - s4) >> 2);
+      if constexpr (rel_vec) {
+        const int64_t vec_row = rel_vec_row(prm.rel, b, h);
+        rel_vec_keys = prm.rel.vec + vec_row * prm.rel.vec_width;
+        const int4 extent = __ldg(prm.rel.vec_extent + vec_row);
+        vec_first = extent.y * kStepN;
+        vec_last = extent.z * kStepN;
+        bias_next = __ldg(rel_vec_keys + key0 + r);
+      }
     }
-    auto load_vec = [&](int col) {
-      if constexpr (rel_bias) return scaled_or_masked(load_elem<kBf16>(bias_vec, col, prm.ex.bias_f32));
-      else return load_bias1<kBf16>(prm.ex, bias_vec, col);
-    };
     if constexpr (vec_bias) {
       bias_vec = static_cast<const uint8_t*>(prm.ex.bias) +
                  (b * prm.ex.bias_stride_b + h * prm.ex.bias_stride_h) * (prm.ex.bias_f32 ? 4 : 2);
       const int col = key0 + r;
-      bias_next = (col < prm.Sk) ? load_vec(col) : 0.f;
+      bias_next = (col < prm.Sk) ? load_bias1<kBf16>(prm.ex, bias_vec, col) : 0.f;
     }
 
     // S of the next step is normally complete long before it is needed: polled once while the
@@ -277,9 +290,19 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     // Stages the row-independent bias of the key tile that step `tn` starts.
     auto stage_vec_bias = [&](int tn) {
       const int j = tn >> 1;
+      if constexpr (rel_vec) {
+        // Only where it is not zero.  A buffer is rewritten two key tiles later, when S of a step after its last
+        // reader's is complete.
+        const int key = key0 + j * tile_dir, next = key + tile_dir;
+        const bool here = key < vec_last && key + kBlockN > vec_first;
+        if (here) sb[(j & 1) * 128 + r] = bias_next;
+        if (next >= 0 && next < vec_last && next + kBlockN > vec_first) bias_next = __ldg(rel_vec_keys + next + r);
+        if (here) named_barrier_sync(1 + s, 128);
+        return;
+      }
       sb[(j & 1) * 128 + r] = bias_next;
       const int col = key0 + (j + 1) * tile_dir + r;  // of the key tile after this one (there may be none)
-      bias_next = (col >= 0 && col < prm.Sk) ? load_vec(col) : 0.f;
+      bias_next = (col >= 0 && col < prm.Sk) ? load_bias1<kBf16>(prm.ex, bias_vec, col) : 0.f;
       // a buffer is rewritten two key tiles later, behind the barrier of the tile between
       named_barrier_sync(1 + s, 128);
     };
@@ -314,41 +337,21 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       const bool need_mask = (k0n + kStepN > prm.Sk) || (prm.causal && k0n + kStepN - 1 > q0 + q_off);
       // relative positions of the warp's 32 rows and the step's keys: d_last - 94 to d_last
       const int d_last = k0n + kStepN - 1 - warp_row;
+      const int half = (tn & 1) ^ first;  // of the key tile
+      const bool step_vec = rel_vec && k0n < vec_last && k0n >= vec_first;
       const RelSide side = rel_bias ? rel_side(prm.rel, d_last - (kStepN + 30), d_last) : kRelNear;
       if constexpr (rel_bias) {
         exp_add = side == kRelLeft ? rel_left : side == kRelRight ? rel_right : 0.f;
-        exp_scale = vec_bias || side == kRelNear ? 1.f : prm.scale_log2;
+        exp_scale = step_vec || side == kRelNear ? 1.f : prm.scale_log2;
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         tmem_ld_wait(sr[c]);
         if ((warp & 3) == 0 && tn > 0) trace_event(prm, s, tn - 1, c == 0 ? 1 : 4);  // loads in
         if constexpr (rel_bias) {
-          const float4* bv = reinterpret_cast<const float4*>(sb + ((tn >> 1) & 1) * 128 + ((tn & 1) ^ first) * kStepN + c * 32);
-          if (side == kRelNear) {
-            const float4* const rv = rel_row + (k0n >> 2) + c * 8;
-            float4 r4[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) r4[i] = __ldg(rv + i);
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              float2 lo = make_float2(r4[i >> 2].x, r4[i >> 2].y), hi = make_float2(r4[i >> 2].z, r4[i >> 2].w);
-              if constexpr (vec_bias) {
-                const float4 v4 = bv[i >> 2];
-                lo = __fadd2_rn(lo, make_float2(v4.x, v4.y));
-                hi = __fadd2_rn(hi, make_float2(v4.z, v4.w));
-              }
-              add_bias2(c, i, lo);
-              add_bias2(c, i + 2, hi);
-            }
-          } else if constexpr (vec_bias) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 v4 = bv[i >> 2];
-              add_bias2(c, i, make_float2(v4.x, v4.y));
-              add_bias2(c, i + 2, make_float2(v4.z, v4.w));
-            }
-          }
+          const float* const bv = sb + ((tn >> 1) & 1) * 128 + half * kStepN + c * 32;
+          add_rel_bias<false>(sr[c], prm.scale_log2, side == kRelNear, rel_row + ((k0n + c * 32) >> 2),
+                       step_vec ? reinterpret_cast<const float4*>(bv) : nullptr);
         } else if constexpr (vec_bias) {
           const float4* bv = reinterpret_cast<const float4*>(sb + ((tn >> 1) & 1) * 128 + ((tn & 1) ^ first) * kStepN + c * 32);
 #pragma unroll
@@ -406,7 +409,7 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     };
 
     // prologue: scores of the first step; their row maximum is the first reference maximum
-    if constexpr (vec_bias) stage_vec_bias(first);
+    if constexpr (vec_bias || rel_vec) stage_vec_bias(first);
     if constexpr (mat_bias16) fetch_mat_bias(first);
     mbar_wait(bar_s_full + 2 * s + first, 0, cta_abort, dstat, FO_STATUS_TIMEOUT_MMA);
     tcgen05_fence_after_sync();
@@ -504,7 +507,7 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         // S of step t + 1 was issued when P of step t - 1 was handed over: complete by now as a
         // rule.  Its loads go out behind the P stores; the score registers are free, everything
         // of step t is in pr.
-        if (vec_bias && u == 1) stage_vec_bias(t + 1);
+        if ((vec_bias || rel_vec) && u == 1) stage_vec_bias(t + 1);
         if constexpr (mat_bias16) fetch_mat_bias(t + 1);
         if (mat_bias && bias_row != nullptr && t + 2 < end) {
           const int c0 = step_key(t + 2, first, key0);

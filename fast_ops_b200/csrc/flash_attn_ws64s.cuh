@@ -18,7 +18,8 @@
 // V in the order the MMA warp consumes them: K(0) K(1) V(0) K(2) V(1) K(3) ... (step t's P V
 // needs V(t), and S of step t + 2 is issued right behind it); a slot is released as soon as the
 // instruction that reads it has been issued, so four slots of 16 KB keep about two steps of loads in
-// flight.  Plain attention only (no bias, no dropout).  No register reallocation between the roles
+// flight.  Plain attention, or with a relative position bias (kExt kFwdRelBias, with or without
+// kFwdVecBias); no other bias, no dropout.  No register reallocation between the roles
 // (setmaxnreg): the CTA's six warps do not make whole warpgroups, and a version that used it did
 // not return; the softmax code fits the 168 registers of the launch bound with 84 bytes of spills.
 #pragma once
@@ -43,10 +44,24 @@ struct Ws64sConfig {
   // barriers: q_full, kv_full/empty per stage, s_full[2], p_full[2], o_full, o_done
   static constexpr int kNumBars = 1 + 2 * kStages + 2 + 2 + 1 + 1;
   static constexpr int kOffMisc = kOffBars + kNumBars * 8;
-  static constexpr int kSmemBytes = kOffMisc + 32 + 1024 /* alignment slack */;
+  static constexpr int kOffBias = (kOffMisc + 32 + 15) & ~15;  // [2][64] float: a vector bias beside a relative one
+  static constexpr int kOffRel = kOffBias + 2 * kStepN * 4;    // RelHead
+  static constexpr int kOffRelVector = kOffRel + 32;            // the head's four copies of the bias vector
+  static constexpr int kSmemBytes = kOffRelVector + 1024 /* alignment slack */;
+  // Longest copy of the vector that leaves room for two CTAs on an SM.
+  static constexpr int kMaxRelStride = (228 * 1024 / 2 - 1024 - kSmemBytes) / 16;
   static constexpr uint32_t kTmemCols = 256;
   static constexpr uint32_t kColS = 0, kColO = 128;
 };
+// What a CTA's steps need of a relative bias beside the kernel's arguments.  Kept in shared memory: in registers it
+// is spilled, and beside two CTAs of head_dim 128 the first-level cache does not hold the spills (us per launch,
+// B2 H16 S4096 D128 causal with key padding: TODO).
+struct RelHead {
+  float left, right;         // the two far constants
+  int vec_first, vec_last;   // 64-key steps between which the vector bias is not zero
+  int vec_row;               // this head's row of it
+};
+
 // two CTAs per SM: 2 x (dynamic + 1 KiB reserved) must fit in the SM's 228 KiB
 static_assert(2 * (Ws64sConfig<128>::kSmemBytes + 1024) <= 228 * 1024, "two CTAs of the D=128 kernel per SM");
 
@@ -54,7 +69,7 @@ static_assert(2 * (Ws64sConfig<128>::kSmemBytes + 1024) <= 228 * 1024, "two CTAs
 // tile-major with the last query tile (the most keys under a causal mask) first.
 // kMma: the head_dim the matmuls compute, at most the tiles' width D (the columns between are zeros;
 // B1 H48 Sq1000 Sk1531 D80: 51 to 49.5 us with 96 instead of 128 columns computed).
-template <int D, bool kBf16, int kMma = D>
+template <int D, bool kBf16, int kMma = D, int kExt = 0>
 __global__ void __launch_bounds__(192, 2)
 attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const AttnParams prm) {
@@ -79,6 +94,7 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Cfg::kOffMisc);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* skip = cta_abort + 1;
+  RelHead* const rel_head = reinterpret_cast<RelHead*>(smem + Cfg::kOffRel);
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -94,7 +110,10 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   const int h = bh - b * prm.H;
   const int hk = prm.kv_head_bcast ? 0 : h;  // head coordinate of K and V
   const int q0 = q_tile * kBlockM;
-  const int vis = prm.causal ? min(prm.Sk, q0 + kBlockM) : prm.Sk;  // keys this tile sees
+  constexpr bool rel_bias = (kExt & kFwdRelBias) != 0, rel_vec = rel_bias && (kExt & kFwdVecBias) != 0;
+  const int q_off = rel_bias ? prm.rel.offset : 0;  // query row i stands at key position i + q_off
+  const int keys = rel_bias ? rel_keys(prm.rel, b, h, prm.Sk) : prm.Sk;
+  const int vis = prm.causal ? min(keys, q0 + kBlockM + q_off) : keys;  // keys this tile sees
   const int T = (vis + kStepN - 1) / kStepN;                       // 64-key steps, >= 1
   // ring entries: K(0), K(1) if it exists, then per step t: V(t), K(t + 2) if it exists
   const int n_entries = 2 * T;
@@ -154,6 +173,16 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     tmem_alloc(tmem_slot, Cfg::kTmemCols);
     tmem_relinquish_alloc_permit();
   }
+  if (rel_bias && tid == 0) {
+    RelHead head = {rel_value(prm.rel, h, -prm.rel.zero), rel_value(prm.rel, h, prm.rel.width), 0, 0, 0};
+    if constexpr (rel_vec) {
+      head.vec_row = static_cast<int>(rel_vec_row(prm.rel, b, h));
+      const int4 extent = __ldg(prm.rel.vec_extent + head.vec_row);
+      head.vec_first = extent.y;
+      head.vec_last = extent.z;
+    }
+    *rel_head = head;
+  }
   tcgen05_fence_before_sync();
   __syncthreads();
   tcgen05_fence_after_sync();
@@ -167,7 +196,24 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t tS_tile = tmem_base + Cfg::kColS + lane_base;
     const uint32_t tO = tmem_base + Cfg::kColO + lane_base;
-    const float exp_scale = prm.scale_log2;
+    // a relative bias: see flash_attn_ws64r.cuh
+    float exp_scale = prm.scale_log2, exp_add = 0.f;
+    float* const sb = reinterpret_cast<float*>(smem + Cfg::kOffBias);
+    float* const s_rel = reinterpret_cast<float*>(smem + Cfg::kOffRelVector);
+    int rel_x = 0;  // where this row's bias of key 0 would be in its copy of the vector
+    if constexpr (rel_bias) {
+      const int x = prm.rel.zero - row - q_off, s4 = x & 3;
+      rel_x = s4 * prm.rel.stride + (x - s4);
+      const float* const src = prm.rel.values + static_cast<int64_t>(h) * 4 * prm.rel.stride;
+      for (int i = r; i < prm.rel.stride; i += 128) cp_async16(s_rel + 4 * i, src + 4 * i);
+    }
+    // Copies step tn's values into their buffer, asynchronously, where they are not zero.
+    auto fetch_vec = [&](int tn) {
+      if (r < kStepN / 4 && tn < rel_head->vec_last && tn >= rel_head->vec_first && tn < T)
+        cp_async16(sb + (tn & 1) * kStepN + 4 * r,
+                   prm.rel.vec + static_cast<int64_t>(rel_head->vec_row) * prm.rel.vec_width + tn * kStepN + 4 * r);
+    };
+    if constexpr (rel_vec) fetch_vec(0);
     float m_run = -INFINITY, l_run = 0.f;
     uint32_t sr[2][32];  // scores of the current step
 
@@ -175,20 +221,44 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     // Waits for those loads and applies the masks in place.
     auto prep_loads = [&](int tn) {
       const int k0n = tn * kStepN;
-      const bool need_mask = (k0n + kStepN > prm.Sk) || (prm.causal && k0n + kStepN - 1 > q0);
+      const bool need_mask = (k0n + kStepN > prm.Sk) || (prm.causal && k0n + kStepN - 1 > q0 + q_off);
+      // relative positions of the warp's 32 rows and the step's keys: d_last - 94 to d_last
+      const int d_last = k0n + kStepN - 1 - (q0 + warp * 32 + q_off);
+      const bool step_vec = rel_vec && tn < rel_head->vec_last && tn >= rel_head->vec_first;
+      if constexpr (rel_vec) {
+        // Behind the barrier no thread reads the values of the step before (without one here there are none),
+        // whose buffer the next step's go to.
+        if (step_vec) {
+          cp_async_wait_all();
+          named_barrier_sync(1, 128);
+        }
+        fetch_vec(tn + 1);
+      }
+      const RelSide side = rel_bias ? rel_side(prm.rel, d_last - (kStepN + 30), d_last) : kRelNear;
+      if constexpr (rel_bias) {
+        exp_add = side == kRelNear ? 0.f : side == kRelLeft ? rel_head->left : rel_head->right;
+        exp_scale = step_vec || side == kRelNear ? 1.f : prm.scale_log2;
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         tmem_ld_wait(sr[c]);
+        if constexpr (rel_bias)
+          add_rel_bias<true>(sr[c], prm.scale_log2, side == kRelNear,
+                             reinterpret_cast<const float4*>(s_rel + (rel_x + k0n + c * 32)), step_vec ? reinterpret_cast<const float4*>(sb + (tn & 1) * kStepN + c * 32) : nullptr);
         if (need_mask) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const int col = k0n + c * 32 + i;
-            if (col >= prm.Sk || (prm.causal && col > row)) sr[c][i] = 0xff800000u;  // -inf
+            if (col >= prm.Sk || (prm.causal && col > row + q_off)) sr[c][i] = 0xff800000u;  // -inf
           }
         }
       }
     };
 
+    if constexpr (rel_bias) {  // every thread's part of the vector is there
+      cp_async_wait_all();
+      named_barrier_sync(1, 128);
+    }
     // prologue: scores of step 0; their row maximum is the first reference maximum
     mbar_wait(bar_s_full + 0, 0, cta_abort, dstat, FO_STATUS_TIMEOUT_MMA);
     tcgen05_fence_after_sync();
@@ -207,7 +277,8 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
           mxd = max3(mxd, __uint_as_float(sr[c][i + 6]), __uint_as_float(sr[c][i + 7]));
         }
       }
-      m_run = fmaxf(fmaxf(mxa, mxb), fmaxf(mxc, mxd)) * exp_scale;
+      const float mx = fmaxf(fmaxf(mxa, mxb), fmaxf(mxc, mxd));
+      m_run = rel_bias ? fmaf(mx, exp_scale, exp_add) : mx * exp_scale;
     }
 
     // As in flash_attn_ws64.cuh: a step's exponentials are taken against the reference maximum the
@@ -216,7 +287,8 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     for (int t = 0; t < T; ++t) {
       const int u = t & 1;
       const uint32_t tS = tS_tile + u * kStepN;
-      const float neg_m = (m_run == -INFINITY) ? 0.f : -m_run;
+      float neg_m = (m_run == -INFINITY) ? 0.f : -m_run;
+      if constexpr (rel_bias) neg_m += exp_add;
       const float2 sc2 = make_float2(exp_scale, exp_scale);
       float2 acc0, acc1;
       uint32_t pr[2][16];
@@ -246,7 +318,8 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         }
       };
       exp_pass(neg_m, true);
-      const float m_cand = fmaxf(m_run, fmaxf(mxa, mxb) * exp_scale);
+      const float mx = fmaxf(mxa, mxb);
+      const float m_cand = fmaxf(m_run, rel_bias ? fmaf(mx, exp_scale, exp_add) : mx * exp_scale);
       const bool grow = m_cand - m_run > kRescaleThreshold;  // false when both are -inf (NaN)
       float alpha = 1.f;
       if (__any_sync(0xffffffffu, grow)) {
@@ -254,7 +327,7 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
         const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
         alpha = grow ? fast_exp2(m_run - m_use) : 1.f;
         m_run = m_new;
-        exp_pass(-m_use, false);
+        exp_pass(rel_bias ? exp_add - m_use : -m_use, false);
         if (t > 0) {
           // O holds the sum up to step t - 1 once that step's P V has finished (the P V two steps
           // back is known to have finished, since S of this step exists: the phase is unambiguous);
@@ -407,12 +480,14 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   if (warp == 4) tmem_dealloc(tmem_base, Cfg::kTmemCols);
 }
 
-template <int D, bool kBf16, int kMma = D>
+template <int D, bool kBf16, int kMma = D, int kExt = 0>
 int launch_ws64s(const CUtensorMap& tq, const CUtensorMap& tk_half, const CUtensorMap& tv_half, const AttnParams& prm,
                  cudaStream_t stream) {
-  auto kernel = attn_fwd_ws64s_kernel<D, kBf16, kMma>;
-  constexpr int smem = Ws64sConfig<D>::kSmemBytes;
-  cudaError_t ea = ensure_dynamic_smem<attn_fwd_ws64s_kernel<D, kBf16, kMma>>(smem, prm.device);
+  auto kernel = attn_fwd_ws64s_kernel<D, kBf16, kMma, kExt>;
+  constexpr int most = Ws64sConfig<D>::kSmemBytes + (kExt != 0 ? 16 * Ws64sConfig<D>::kMaxRelStride : 0);
+  const int smem = Ws64sConfig<D>::kSmemBytes + (kExt != 0 ? 16 * prm.rel.stride : 0);
+  if (smem > most) return fail(FO_ERR_UNSUPPORTED, "the bias vector does not fit this kernel");
+  cudaError_t ea = ensure_dynamic_smem<attn_fwd_ws64s_kernel<D, kBf16, kMma, kExt>>(most, prm.device);
   if (ea != cudaSuccess)
     return fail(FO_ERR_CUDA, "cudaFuncSetAttribute(shared memory %d) failed: %s", smem, cudaGetErrorString(ea));
   const int64_t blocks = static_cast<int64_t>(prm.num_q_tiles) * prm.B * prm.H;

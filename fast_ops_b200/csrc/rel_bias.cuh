@@ -9,7 +9,13 @@
 // tiles near the diagonal read it at all; its ends reach kRelMargin further, which is more than a warp's
 // part of such a tile can.  A thread reads neighbouring values from a place of its own, 16 bytes at a time:
 // the vector is there four times, copy s shifted by s values, so that one of them is aligned for it
-// (64 values by 16 loads instead of 64: forward B8 H12 S1024 D64 TODO).
+// (64 values by 16 loads instead of 64).  The copies are 8 banks apart, so that from shared memory eight
+// threads read 32 banks.
+//
+// A vector bias beside it (key padding, as a rule) is brought into fp32 times log2(e) too, one row for each
+// batch and head that has its own, with what lets the kernels pass over most of it: the end of the keys that
+// are not masked, behind which nothing is computed, and the 64-key steps from the first value that is not 0 to
+// the last one before that end.
 #pragma once
 
 #include <cstdint>
@@ -54,6 +60,10 @@ struct RelBias {
   float* acc;
   float2* tile_sums;
   int width, zero, stride;
+  const float* vec;          // [rows][rel_vec_width], or null without a vector bias
+  const int4* vec_extent;    // [rows]: (keys up to the last one not masked, first step with a bias, step after the last, 0)
+  int vec_row_b, vec_row_h;  // row of (b, h): b * vec_row_b + h * vec_row_h
+  int vec_width;
   int far_left, far_right;
   int offset;
   int num_buckets;
@@ -69,6 +79,47 @@ __device__ __forceinline__ RelSide rel_side(const RelBias& rel, int first, int l
 __device__ __forceinline__ float rel_value(const RelBias& rel, int h, int d) {
   const int x = min(max(d, -rel.zero), rel.width - 1 - rel.zero) + rel.zero;
   return __ldg(rel.values + static_cast<int64_t>(h) * 4 * rel.stride + x);
+}
+
+// Row of the vector bias, and the keys that a head computes: `keys`, or those up to the last one not masked, but
+// at least one (whose score is -inf if it is masked too).
+__device__ __forceinline__ int64_t rel_vec_row(const RelBias& rel, int b, int h) {
+  return static_cast<int64_t>(b) * rel.vec_row_b + static_cast<int64_t>(h) * rel.vec_row_h;
+}
+__device__ __forceinline__ int rel_keys(const RelBias& rel, int b, int h, int keys) {
+  return rel.vec == nullptr ? keys : min(keys, max(__ldg(&rel.vec_extent[rel_vec_row(rel, b, h)].x), 1));
+}
+
+// Keys of a row of `vec`: whole key tiles.
+__host__ __device__ inline int rel_vec_width(int Sk) { return (Sk + 127) / 128 * 128; }
+
+// Scales 32 scores and adds the bias where it is not the same for all of them: the relative bias near the
+// diagonal (`near`, this thread's values at `rel`, in shared memory or not), the vector bias where it is not zero
+// (`vec`, in shared memory, or null).
+template <bool kShared>
+__device__ __forceinline__ void add_rel_bias(uint32_t (&s)[32], float scale, bool near, const float4* rel, const float4* vec) {
+  auto add = [&](int i, float2 bias) {
+    const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(scale, scale), bias);
+    s[i] = __float_as_uint(x.x);
+    s[i + 1] = __float_as_uint(x.y);
+  };
+  if (near) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 r = kShared ? rel[i] : __ldg(rel + i);
+      add(4 * i, make_float2(r.x, r.y));
+      add(4 * i + 2, make_float2(r.z, r.w));
+    }
+    scale = 1.f;
+  }
+  if (vec != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 v = vec[i];
+      add(4 * i, make_float2(v.x, v.y));
+      add(4 * i + 2, make_float2(v.z, v.w));
+    }
+  }
 }
 
 // Where a thread finds the values from x on (x >= 0): 16-byte aligned, for head h.

@@ -63,9 +63,10 @@ def _starts_array(num_buckets: int, max_distance: int, bidirectional: bool):
 
 
 @lru_cache(maxsize=256)
-def _workspace_bytes(H: int, M: int, N: int, num_buckets: int, max_distance: int, bidirectional: bool, offset: int) -> int:
+def _workspace_bytes(H: int, M: int, N: int, num_buckets: int, max_distance: int, bidirectional: bool, offset: int,
+                     bias_rows: int) -> int:
     starts, n = _starts_array(num_buckets, max_distance, bidirectional)
-    size = _lib.load().fo_rel_attn_workspace(H, M, N, starts, n, int(bidirectional), offset)
+    size = _lib.load().fo_rel_attn_workspace(H, M, N, starts, n, int(bidirectional), offset, bias_rows)
     _lib.check(-1 if size < 0 else 0)
     return size
 
@@ -122,17 +123,19 @@ class _Call:
         if bias is not None and bias.dim() == 4 and bias.shape[2] != 1:
             raise RuntimeError("beside a relative bias, bias must be (1 or B, 1 or H, 1, N): the same for every query")
         kept, ptr, strides, code = _prepare_bias(bias, Q, self.B, self.H, self.M, self.N)
+        rows = 0
         if strides is not None:
             strides[2] = 0  # a single query row's stride says nothing
-        return kept, (ptr, strides, code)
+            rows = (self.B if strides[0] else 1) * (self.H if strides[1] else 1)
+        return kept, rows, (ptr, strides, code)
 
     def forward(self, Q: Tensor, K: Tensor, V: Tensor, table: Tensor, bias: Optional[Tensor], lse: bool):
         """(O, LSE or None, the expanded bias)."""
         O = torch.empty_like(Q, memory_format=torch.contiguous_format)
         lse_t = Q.new_empty((self.B, self.H, self.M), dtype=torch.float32) if lse else None
-        workspace = torch.empty(_workspace_bytes(self.H, self.M, self.N, *self.key, self.offset), dtype=torch.uint8,
-                                device=self.device)
-        kept, bias_args = self.bias(bias, Q)
+        kept, rows, bias_args = self.bias(bias, Q)
+        workspace = torch.empty(_workspace_bytes(self.H, self.M, self.N, *self.key, self.offset, rows),
+                                dtype=torch.uint8, device=self.device)
         ts = table.stride()
         _lib.check(_lib.load().fo_rel_attn_fwd(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), lse_t.data_ptr() if lse else None, self.B, self.H, self.M, self.N, self.D,
@@ -167,7 +170,7 @@ class _Call:
         scratch = torch.empty(rows * (self.D + 1) + partials, dtype=torch.float32, device=self.device)
         dq_accum = scratch.data_ptr()
         partial_sums = dq_accum + 4 * rows * self.D  # a multiple of 32 bytes on, since D is one of 8
-        kept, bias_args = self.bias(bias, Q)
+        kept, _, bias_args = self.bias(bias, Q)
         _lib.check(lib.fo_rel_attn_bwd(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), dO.data_ptr(), LSE.data_ptr(), dQ.data_ptr(),
             dK.data_ptr(), dV.data_ptr(), None if dtable is None else dtable.data_ptr(), dq_accum,

@@ -160,6 +160,8 @@ int fo_flash_attn_bwd_ex(const void* q, const void* k, const void* v, const void
  *   query_offset : key position of query row 0, in [0, 2^29].
  *   workspace  : device memory of fo_rel_attn_workspace(...) bytes, 16-byte aligned.  The forward writes
  *                the expanded bias there; the backward must be given it as the forward left it.
+ *                bias_rows: 0 without `bias`, otherwise (B, or 1 if bias_strides[0] is 0) times (H, or
+ *                1 if bias_strides[1] is 0).
  *   bias       : as in fo_flash_attn_fwd_ex, but the same for every query row: bias_strides[2] = 0.
  *                Entries of -1e6 and below mask like -inf, in the table too.
  *   dtable     : NULL (no gradient of the table), or (n_buckets, H) dense, of table_dtype.
@@ -170,7 +172,8 @@ int fo_flash_attn_bwd_ex(const void* q, const void* k, const void* v, const void
  * there is an lse (a backward may follow).
  * The workspace functions return -1 for arguments that the calls refuse.
  */
-int64_t fo_rel_attn_workspace(int H, int Sq, int Sk, const int* starts, int n_starts, int two_sided, int query_offset);
+int64_t fo_rel_attn_workspace(int H, int Sq, int Sk, const int* starts, int n_starts, int two_sided, int query_offset,
+                              int64_t bias_rows);
 int64_t fo_rel_attn_bwd_workspace(int B, int H, int Sq, int Sk, int D, int num_buckets, int dropout);
 int fo_rel_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
                     int B, int H, int Sq, int Sk, int D,

@@ -441,3 +441,34 @@ def test_refusals(cuda_device):
         with pytest.raises(RuntimeError):
             bad()
     assert relative_bucket_starts(32, 128, True)[-1] == 91
+
+
+@pytest.mark.parametrize("D,causal", [(64, False), (128, False), (64, True), (128, True)])
+@pytest.mark.parametrize("dropout_p", [0.0, 0.1])
+def test_masks_with_holes_and_ragged_ends(D, causal, dropout_p, cuda_device):
+    """Keys masked in front, in the middle and at the end, whole key tiles of them, and values that are not masks."""
+    B, H, M, N = 4, 2, 330, 700
+    Q, K, V, table, dO = make(B, H, M, N, D, BF, 32, seed=2)
+    bias = torch.zeros(B, 1, 1, N, device="cuda")
+    bias[0, ..., 300:] = -math.inf
+    bias[1, ..., :200] = -math.inf
+    bias[1, ..., 250:520] = -math.inf
+    bias[2, ..., 0] = 1.5
+    bias[2, ..., 699] = -2.0
+    bias[3] = torch.linspace(-3, 3, N, device="cuda")
+    keep = dropout_mask(dropout_p, B, H, M, N, Q.device, rng=(5, 0)) if dropout_p else None
+    check_train(Q, K, V, table, dO, keep=keep, max_distance=128, bidirectional=not causal, causal=causal, bias=bias,
+                dropout_p=dropout_p, rng=(5, 0), query_offset=370 if causal else 0)
+
+
+@pytest.mark.parametrize("impl", ["ws64", "ws64s"])
+@pytest.mark.parametrize("D,dtype", [(64, BF), (128, HF), (96, BF)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_both_forward_kernels(impl, D, dtype, causal, cuda_device):
+    Q, K, V, table, dO = make(2, 3, 420, 420, D, dtype, 32, seed=6)
+    L.attn_configure(impl=impl)
+    try:
+        for bias in (None, padding(2, 420, (300, 64))):
+            check_train(Q, K, V, table, dO, max_distance=128, bidirectional=not causal, causal=causal, bias=bias)
+    finally:
+        L.attn_configure(impl="auto")
