@@ -354,12 +354,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const int64_t rel_sums_step = static_cast<int64_t>(gridDim.x) * kCW;
     const int warp_key = k0 + (warp & 3) * 32 - q_off;  // query row that the warp's first key stands beside
     if constexpr (rel_bias) {
-      rel_left = rel_value(prm.rel, h, -prm.rel.zero);
-      rel_right = rel_value(prm.rel, h, prm.rel.width);
+      rel_left = rel_value(prm.rel, h, -prm.rel.zero) * prm.scale_log2;
+      rel_right = rel_value(prm.rel, h, prm.rel.width) * prm.scale_log2;
       // values of query rows 3 to 0, which may lie behind the vector; those read do not
       const int x = prm.rel.zero + key - q_off - 3, s4 = x & 3;
       rel_col = rel_vector(prm.rel, h, s4) + ((x - s4) >> 2);
-      if (prm.rel.vec != nullptr) bias_key = __ldg(prm.rel.vec + rel_vec_row(prm.rel, b, h) * prm.rel.vec_width + key);
+      if (prm.rel.vec != nullptr) bias_key = __ldg(prm.rel.vec + rel_vec_row(prm.rel, b, h) * prm.rel.vec_width + key) * prm.scale_log2;
       if (prm.rel.acc != nullptr) {
         rel_acc = prm.rel.acc + ((static_cast<int64_t>(bh) * gridDim.x + j) * kCW + warp) * prm.rel.num_buckets;
         for (int x = lane; x < prm.rel.num_buckets; x += 32) rel_acc[x] = 0.f;
@@ -400,7 +400,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                                 prm.Sq - q, bias_v);
       };
       if constexpr (mat_bias) load_bias_piece(0);
-      const float rel_far = bias_key + (side == kRelLeft ? rel_left : rel_right);
+      const float rel_far = rel_near ? bias_key : bias_key + (side == kRelLeft ? rel_left : rel_right);
       mbar_wait(bar_lse_full + Cfg::par(it), Cfg::phase(it), cta_abort, dstat, FO_STATUS_TIMEOUT_TMA);
       mbar_wait(bar_s_full, it & 1, cta_abort, dstat, FO_STATUS_TIMEOUT_MMA);
       tcgen05_fence_after_sync();
@@ -409,39 +409,58 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       uint32_t sr[kPieces][32];
 #pragma unroll
       for (int cc = 0; cc < kPieces; ++cc) tmem_ld32(tS + cc * 32, sr[cc]);
-      // with a relative bias the parts near the diagonal have a loop of their own
-      auto exponentials = [&](auto near) {
+      // with a relative bias, what few parts need comes before the exponentials, behind one branch
+      if constexpr (rel_bias) {
+#pragma unroll
+        for (int cc = 0; cc < kPieces; ++cc) tmem_ld_wait(sr[cc]);
+        if (rel_near || need_mask) {
+#pragma unroll
+          for (int cc = 0; cc < kPieces; ++cc) {
+            if (rel_near) {
+              // this key's bias for 32 consecutive query rows, four at a time in descending order
+              const float4* const rv = rel_col - ((qc0 + cc * 32) >> 2);
+#pragma unroll
+              for (int x = 0; x < 32; x += 4) {
+                const float4 u = __ldg(rv - (x >> 2));
+                const float bv[4] = {u.w, u.z, u.y, u.x};
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sr[cc][x + y] = __float_as_uint(__uint_as_float(sr[cc][x + y]) + bv[y]);
+              }
+            }
+            if (need_mask) {
+#pragma unroll
+              for (int x = 0; x < 32; ++x) {
+                const int q = qc0 + cc * 32 + x;
+                if (!key_ok || (prm.causal && key > q + q_off)) sr[cc][x] = 0xff800000u;  // -inf
+              }
+            }
+          }
+        }
+      }
+      auto exponentials = [&]() {
 #pragma unroll
         for (int cc = 0; cc < kPieces; ++cc) {
           const float* nl = sNegLse + (it & (Cfg::kSlots - 1)) * 128 + part * kCols + cc * 32;
-          tmem_ld_wait(sr[cc]);
+          if constexpr (!rel_bias) tmem_ld_wait(sr[cc]);
           if constexpr (mat_bias) {
             if (cc > 0) load_bias_piece(cc);
           }
-          // this key's bias for 32 consecutive query rows, four at a time in descending order
-          const float4* const rv = rel_col - ((qc0 + cc * 32) >> 2);
 #pragma unroll
           for (int x = 0; x < 32; x += 4) {
             const float4 t = *reinterpret_cast<const float4*>(nl + x);  // broadcast read
             const float nlv[4] = {t.x, t.y, t.z, t.w};
-            float bv[4] = {};
-            if constexpr (near.value) {
-              const float4 u = __ldg(rv - (x >> 2));
-              bv[0] = u.w + bias_key; bv[1] = u.z + bias_key; bv[2] = u.y + bias_key; bv[3] = u.x + bias_key;
-            }
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const float sv = __uint_as_float(sr[cc][x + y]);
               float e;
               if constexpr (mat_bias) e = fmaf(sv, prm.scale_log2, bias_v[x + y]) + nlv[y];
-              else if constexpr (near.value) e = fmaf(sv, prm.scale_log2, bv[y]) + nlv[y];
               else if constexpr (rel_bias) e = fmaf(sv, prm.scale_log2, rel_far) + nlv[y];
               else if constexpr (vec_bias) e = fmaf(sv, prm.scale_log2, bias_key) + nlv[y];
               else e = fmaf(sv, prm.scale_log2, nlv[y]);
               sr[cc][x + y] = __float_as_uint(fast_exp2(e));
             }
           }
-          if (need_mask) {
+          if (!rel_bias && need_mask) {
 #pragma unroll
             for (int x = 0; x < 32; ++x) {
               const int q = qc0 + cc * 32 + x;
@@ -450,12 +469,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         }
       };
-      if constexpr (rel_bias) {
-        if (rel_near) exponentials(std::true_type{});
-        else exponentials(std::false_type{});
-      } else {
-        exponentials(std::false_type{});
-      }
+      exponentials();
       if (warp == 0) bwd_trace(prm, 0, it, 4);
       float p_sum = 0.f;
       if constexpr (rel_bias) {

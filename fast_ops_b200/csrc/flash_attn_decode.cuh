@@ -145,7 +145,7 @@ attn_decode_kernel(const DecodeParams prm, const __grid_constant__ Rel rel) {
 #pragma unroll
     for (int r = 0; r < kHeads; ++r)
       rel_far[r] = scaled_or_masked(load_elem<kBf16>(
-          rel.table, (rel.buckets.n - 1) * rel.stride_bucket + min(h0 + r, prm.H - 1) * rel.stride_head, rel.table_f32));
+          rel.table, (rel.buckets.n - 1) * rel.stride_bucket + min(h0 + r, prm.H - 1) * rel.stride_head, rel.table_f32), 1.4426950408889634f);
   }
 
   uint4 kw[kBatch], vw[kBatch];
@@ -163,9 +163,9 @@ attn_decode_kernel(const DecodeParams prm, const __grid_constant__ Rel rel) {
       for (int r = 0; r < kHeads; ++r) {
         const int h = min(h0 + r, prm.H - 1);
         bias[r] = rel_far[r];
-        if (!far) bias[r] = scaled_or_masked(load_elem<kBf16>(rel.table, bucket * rel.stride_bucket + h * rel.stride_head, rel.table_f32));
+        if (!far) bias[r] = scaled_or_masked(load_elem<kBf16>(rel.table, bucket * rel.stride_bucket + h * rel.stride_head, rel.table_f32), 1.4426950408889634f);
         if (rel.bias != nullptr)
-          bias[r] += scaled_or_masked(load_elem<kBf16>(rel.bias, b * rel.bias_stride_b + h * rel.bias_stride_h + key, rel.bias_f32));
+          bias[r] += scaled_or_masked(load_elem<kBf16>(rel.bias, b * rel.bias_stride_b + h * rel.bias_stride_h + key, rel.bias_f32), 1.4426950408889634f);
       }
     }
     float s[kHeads];

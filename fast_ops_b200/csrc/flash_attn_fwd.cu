@@ -277,6 +277,7 @@ int fo::attn_fwd_impl(const void* q, const void* k, const void* v, void* o, floa
     return fo::fail(FO_ERR_INVALID_ARGUMENT, "head_dim must be a multiple of 8 and <= 128 (got %d)", D);
   const int Dk = D <= 64 ? 64 : 128;  // head_dim the kernel is built for
   FO_REQUIRE(softmax_scale > 0.f && std::isfinite(softmax_scale), "softmax_scale must be positive and finite");
+  FO_REQUIRE(!rel || softmax_scale >= 1e-20f, "with a relative bias softmax_scale must be at least 1e-20 (got %g)", (double)softmax_scale);
   FO_REQUIRE((reinterpret_cast<uintptr_t>(o) & 15) == 0, "o must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
     FO_REQUIRE(o_strides[i] % 8 == 0 && o_strides[i] >= 0, "o: strides must be non-negative multiples of 8 elements");
@@ -307,7 +308,7 @@ int fo::attn_fwd_impl(const void* q, const void* k, const void* v, void* o, floa
     if (int rc = fo::check_layout(k, B, Hkv, Sk, D, k_strides, "k", ks)) return rc;
     if (int rc = fo::check_layout(v, B, Hkv, Sk, D, v_strides, "v", vs)) return rc;
     if (rel && lse != nullptr)  // a backward may follow, whose tile kernels read the expanded bias
-      if (int rc = fo::launch_rel_expand(*rel, *ex, H, Sk, dtype == FO_BF16, static_cast<cudaStream_t>(stream))) return rc;
+      if (int rc = fo::launch_rel_expand(*rel, *ex, H, Sk, softmax_scale, dtype == FO_BF16, static_cast<cudaStream_t>(stream))) return rc;
     return decode(q, k, v, o, lse, B, H, rel ? keys : Sk, D, qs, ks, vs, o_strides, kv_bcast, dtype, softmax_scale, status,
                   rel, ex, info->num_sms, device, static_cast<cudaStream_t>(stream));
   }
@@ -359,11 +360,13 @@ int fo::attn_fwd_impl(const void* q, const void* k, const void* v, void* o, floa
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == FO_BF16;
   if (rel) {
-    if (int rc = fo::launch_rel_expand(*rel, *ex, H, Sk, bf16, s)) return rc;
-    const int64_t pair_items = static_cast<int64_t>((prm.num_q_tiles + 1) / 2) * B * H;
+    if (int rc = fo::launch_rel_expand(*rel, *ex, H, Sk, softmax_scale, bf16, s)) return rc;
+    // One query tile per CTA: the faster one at every shape measured (us, it and the paired kernel: B1 H16 S8192
+    // D128 causal 288 and 304, S16384 1155 and 1149; B2 H16 S4096 D128 157 and 173, padded 175 and 203; B8 H12
+    // S1024 D64 61 and 69).  It keeps the bias vector in shared memory, so buckets that reach too far (distances
+    // of about 300 two-sided at head_dim 128, 800 at 64) take the paired kernel, and so does dropout.
     const int room = Dk == 64 ? fo::Ws64sConfig<64>::kMaxRelStride : fo::Ws64sConfig<128>::kMaxRelStride;
-    const bool half_tiles = !ex->dropout && prm.rel.stride <= room &&
-                            (impl == AttnImpl::kShort64 || (impl == AttnImpl::kAuto && (Dk == 64 || Sk <= 1024 || pair_items <= info->num_sms)));
+    const bool half_tiles = !ex->dropout && prm.rel.stride <= room && impl != AttnImpl::kWarpSpecialized64;
     if (half_tiles) {
       if (int rc = make_tensor_map(&tk, k, dtype, B, Hkv, Sk, D, k_strides, "k", fo::kStepN)) return rc;
       if (int rc = make_tensor_map(&tv, v, dtype, B, Hkv, Sk, D, v_strides, "v", fo::kStepN)) return rc;

@@ -46,7 +46,8 @@ int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
                    bool bf16, cudaStream_t stream);
 int launch_bwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                    const CUtensorMap& tdq, const AttnBwdParams& prm, bool bf16, cudaStream_t stream);
-int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, bool bf16, cudaStream_t stream);
+int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, float softmax_scale, bool bf16,
+                      cudaStream_t stream);
 
 struct DecodeParams;
 int launch_decode_rel(const DecodeParams& prm, const RelArgs& rel, const AttnExtras& ex, int B, int H, int Sk, int D,

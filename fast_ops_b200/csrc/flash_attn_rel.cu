@@ -1,6 +1,8 @@
 // Attention with a learned relative position bias (rel_bias.cuh): entry points, the launches of the tile
 // and decoding kernels built for it, and the two small kernels around them: the bias of a head as a vector
 // over the relative position, and the gradient of the table from the backward's partial sums.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -18,7 +20,7 @@ using fo::RelArgs;
 using fo::RelBias;
 using fo::RelBuckets;
 
-// The bias in the form the tile kernels read: values[h][s][x] = log2(e) * table[bucket(x + s - zero)][h], the
+// The bias in the form the tile kernels read: values[h][s][x] = table[bucket(x + s - zero)][h] / scale, the
 // buckets themselves, and the rows of a vector bias.  The first blocks make the former, 256 positions of one
 // head each; then one block takes each row.
 struct ExpandParams {
@@ -30,6 +32,7 @@ struct ExpandParams {
   int64_t bias_stride_b, bias_stride_h;
   int bias_f32;
   int bias_heads;       // heads of the rows made of it
+  float inv_scale;      // 1 / softmax scale
   int H, Sk, zero, width, stride, value_blocks, vec_width;
   float* values;
   int* bucket_of;
@@ -47,7 +50,7 @@ rel_expand_kernel(const __grid_constant__ ExpandParams prm) {
     if (x >= prm.width) return;
     const int bucket = fo::rel_bucket(prm.buckets, x - prm.zero);
     const float v = fo::scaled_or_masked(
-        fo::load_elem<kBf16>(prm.table, bucket * prm.stride_bucket + h * prm.stride_head, prm.table_f32));
+        fo::load_elem<kBf16>(prm.table, bucket * prm.stride_bucket + h * prm.stride_head, prm.table_f32), prm.inv_scale);
 #pragma unroll
     for (int s = 0; s < 4; ++s)
       if (x >= s) prm.values[(static_cast<int64_t>(h) * 4 + s) * prm.stride + x - s] = v;
@@ -61,7 +64,7 @@ rel_expand_kernel(const __grid_constant__ ExpandParams prm) {
   int end = 0, first = prm.vec_width, last = -1;
 #pragma unroll 4
   for (int key = threadIdx.x; key < prm.vec_width; key += 256) {
-    const float v = key < prm.Sk ? fo::scaled_or_masked(fo::load_elem<kBf16>(prm.bias, src + key, prm.bias_f32)) : 0.f;
+    const float v = key < prm.Sk ? fo::scaled_or_masked(fo::load_elem<kBf16>(prm.bias, src + key, prm.bias_f32), prm.inv_scale) : 0.f;
     dst[key] = v;
     if (v != 0.f) {
       first = min(first, key);
@@ -103,30 +106,39 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return
 // sign, which the far buckets collect over thousands of keys: 0.5 to 1 % of their gradient at S = 4096 to 8192.
 // What the sums over all keys of a block of queries miss zero by is that error's sum over the block; it
 // is put back in proportion to the probability mass that each side holds of the block's queries.
-// One block per head: a warp per (batch, block of kCols queries) for the far sums, then all threads
-// for the sums by bucket, everything in a fixed order and in double.
+// A cluster of kGradCtas blocks per head, whose partial results the first one adds up: a warp per (batch, block of
+// queries) for the far sums, and rows of neighbouring buckets for the sums by bucket.  Everything in a fixed order
+// and in double.  Bound by latency (the sums are a few MB at most): one block per head took 22 us at B16 H12 S512 and
+// 18 at B2 H16 S4096, the cluster TODO.
+constexpr int kGradCtas = 8, kGradWarps = 8;
+
 template <class T>
-__global__ void __launch_bounds__(1024)
+__global__ void __cluster_dims__(kGradCtas, 1, 1) __launch_bounds__(kGradWarps * 32)
 rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, int n_q_tiles, int n_k_tiles, int warps,
                       int causal, float inv_scale) {
-  __shared__ double far[32][2];
-  __shared__ double part[32][33];
-  const int h = blockIdx.x;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ double far[kGradWarps][2];
+  __shared__ double cta_far[2];
+  __shared__ double part[kGradWarps][32];
+  __shared__ double cta_part[2 * fo::kRelMaxStarts];  // sum by bucket of this block's rows
+  const int h = blockIdx.y;
+  const int rank = static_cast<int>(cluster.block_rank());
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int parts = warps / 4, cols = fo::kBlockM / parts;  // four warps share a part's queries
   double left = 0, right = 0;
-  for (int64_t item = warp; item < static_cast<int64_t>(B) * n_q_tiles * parts; item += 32) {
+  for (int64_t item = rank * kGradWarps + warp; item < static_cast<int64_t>(B) * n_q_tiles * parts; item += kGradCtas * kGradWarps) {
     const int p = static_cast<int>(item % parts);
     const int64_t bi = item / parts;
     const int i = static_cast<int>(bi % n_q_tiles);
-    const int64_t bh = bi / n_q_tiles * H + h;
-    const float2* const row = rel.tile_sums + (bh * n_q_tiles + i) * n_k_tiles * warps + p * 4;
-    const int q_first = i * fo::kBlockM + p * cols + rel.offset;  // key position of the part's first query
-    // key tiles that this query tile sees (the backward visits no others)
     const int b = static_cast<int>(bi / n_q_tiles);
+    const float2* const row = rel.tile_sums + ((static_cast<int64_t>(b) * H + h) * n_q_tiles + i) * n_k_tiles * warps + p * 4;
+    const int q_first = i * fo::kBlockM + p * cols + rel.offset;  // key position of the part's first query
+    // key tiles that this query tile sees and that have keys (the backward visits no others)
     int n = rel.vec == nullptr ? n_k_tiles : (fo::rel_keys(rel, b, h, n_k_tiles * fo::kBlockN) + fo::kBlockN - 1) / fo::kBlockN;
     if (causal) n = min(n, (i * fo::kBlockM + fo::kBlockM - 1 + rel.offset) / fo::kBlockN + 1);
     double ds = 0, mass = 0, ds_side[2] = {0, 0}, mass_side[2] = {0, 0};
+#pragma unroll 4
     for (int x = lane; x < n * 4; x += 32) {
       const int key = x * 32;  // key tile x / 4, its quarter x % 4
       const float2 v = row[static_cast<int64_t>(x >> 2) * warps + (x & 3)];
@@ -160,29 +172,47 @@ rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, i
     far[warp][0] = left;
     far[warp][1] = right;
   }
-  __syncthreads();
-  const int left_bucket = rel.bucket_of[0], right_bucket = rel.bucket_of[rel.width - 1];
-  for (int u0 = 0; u0 < rel.num_buckets; u0 += 32) {
+  // rows of the sums by bucket: (batch, key tile, warp), of which this block takes every kGradCtas-th
+  const int per_batch = n_k_tiles * warps;
+  const int64_t rows = static_cast<int64_t>(B) * per_batch;
+  const int nb = rel.num_buckets;
+  for (int u0 = 0; u0 < nb; u0 += 32) {
     const int u = u0 + lane;
     double sum = 0;
-    if (u < rel.num_buckets)
-      for (int b = 0; b < B; ++b) {
-        const float* const p = rel.acc + (static_cast<int64_t>(b) * H + h) * n_k_tiles * warps * rel.num_buckets + u;
-#pragma unroll 4
-        for (int i = warp; i < n_k_tiles * warps; i += 32) sum += static_cast<double>(p[static_cast<int64_t>(i) * rel.num_buckets]);
+    if (u < nb) {
+#pragma unroll 8
+      for (int64_t r = rank * kGradWarps + warp; r < rows; r += kGradCtas * kGradWarps) {
+        const int64_t b = r / per_batch;
+        sum += static_cast<double>(rel.acc[((b * H + h) * per_batch + (r - b * per_batch)) * nb + u]);
       }
+    }
     part[warp][lane] = sum;
     __syncthreads();
-    if (warp == 0 && u < rel.num_buckets) {
-      for (int i = 1; i < 32; ++i) sum += part[i][lane];
-      for (int i = 0; i < 32; ++i) {
-        if (u == left_bucket) sum += far[i][0];
-        if (u == right_bucket) sum += far[i][1];
-      }
-      dtable[static_cast<int64_t>(u) * H + h] = from_f32<T>(static_cast<float>(sum * inv_scale));
+    if (warp == 0 && u < nb) {
+      for (int i = 1; i < kGradWarps; ++i) sum += part[i][lane];
+      cta_part[u] = sum;
     }
     __syncthreads();
   }
+  if (threadIdx.x < 2) {
+    double sum = 0;
+    for (int i = 0; i < kGradWarps; ++i) sum += far[i][threadIdx.x];
+    cta_far[threadIdx.x] = sum;
+  }
+  cluster.sync();
+  if (rank == 0) {
+    const int left_bucket = rel.bucket_of[0], right_bucket = rel.bucket_of[rel.width - 1];
+    for (int u = threadIdx.x; u < nb; u += kGradWarps * 32) {
+      double sum = 0;
+      for (int c = 0; c < kGradCtas; ++c) {
+        sum += cluster.map_shared_rank(cta_part, c)[u];
+        if (u == left_bucket) sum += cluster.map_shared_rank(cta_far, c)[0];
+        if (u == right_bucket) sum += cluster.map_shared_rank(cta_far, c)[1];
+      }
+      dtable[static_cast<int64_t>(u) * H + h] = from_f32<T>(static_cast<float>(sum * inv_scale));
+    }
+  }
+  cluster.sync();  // no block leaves while its shared memory is being read
 }
 
 // Checks of the relative bias's own arguments; fills everything of `rel` but the device pointers of the
@@ -277,7 +307,8 @@ int check_bias_strides(const void* bias, const int64_t* strides) {
 
 namespace fo {
 
-int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, bool bf16, cudaStream_t stream) {
+int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, float softmax_scale, bool bf16,
+                      cudaStream_t stream) {
   ExpandParams prm;
   prm.buckets = rel.buckets;
   prm.table = static_cast<const uint8_t*>(rel.table);
@@ -289,6 +320,7 @@ int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, b
   prm.bias_stride_h = ex.bias_stride_h;
   prm.bias_f32 = ex.bias_f32;
   prm.bias_heads = rel.bias_heads;
+  prm.inv_scale = 1.f / softmax_scale;
   prm.H = H;
   prm.Sk = Sk;
   prm.zero = rel.bias.zero;
@@ -316,6 +348,7 @@ int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
   bf16 ? LAUNCH<DK, true, __VA_ARGS__>(tq, tk, tv, prm, stream) : LAUNCH<DK, false, __VA_ARGS__>(tq, tk, tv, prm, stream)
   const bool wide = prm.d_real > 64, vec = prm.rel.vec != nullptr;
   if (half_tiles) {
+    if (wide && prm.d_real <= 96) return vec ? FO_REL_FORM(launch_ws64s, 128, 96, (kFwdRelBias | kFwdVecBias)) : FO_REL_FORM(launch_ws64s, 128, 96, kFwdRelBias);
     if (wide) return vec ? FO_REL_FORM(launch_ws64s, 128, 128, (kFwdRelBias | kFwdVecBias)) : FO_REL_FORM(launch_ws64s, 128, 128, kFwdRelBias);
     return vec ? FO_REL_FORM(launch_ws64s, 64, 64, (kFwdRelBias | kFwdVecBias)) : FO_REL_FORM(launch_ws64s, 64, 64, kFwdRelBias);
   }
@@ -330,13 +363,14 @@ int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
 
 int launch_bwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                    const CUtensorMap& tdq, const AttnBwdParams& prm, bool bf16, cudaStream_t stream) {
-#define FO_REL_FORM(DK, M) \
-  bf16 ? launch_bwd<DK, true, (M)>(tq, tk, tv, tdo, tdq, prm, stream) : launch_bwd<DK, false, (M)>(tq, tk, tv, tdo, tdq, prm, stream)
+#define FO_REL_FORM(DK, ...) \
+  bf16 ? launch_bwd<DK, true, __VA_ARGS__>(tq, tk, tv, tdo, tdq, prm, stream) : launch_bwd<DK, false, __VA_ARGS__>(tq, tk, tv, tdo, tdq, prm, stream)
   if (prm.d_real > 64) {
-    if (prm.ex.dropout) return FO_REL_FORM(128, kBwdRelBias | kBwdDropout);
+    if (prm.ex.dropout) return FO_REL_FORM(128, (kBwdRelBias | kBwdDropout));
+    if (prm.d_real <= 96) return FO_REL_FORM(128, kBwdRelBias, 96);
     return FO_REL_FORM(128, kBwdRelBias);
   }
-  if (prm.ex.dropout) return FO_REL_FORM(64, kBwdRelBias | kBwdDropout);
+  if (prm.ex.dropout) return FO_REL_FORM(64, (kBwdRelBias | kBwdDropout));
   return FO_REL_FORM(64, kBwdRelBias);
 #undef FO_REL_FORM
 }
@@ -456,7 +490,7 @@ extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, cons
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const float inv = 1.f / softmax_scale;
 #define FO_TABLE_GRAD(T)                                                                                             \
-  rel_table_grad_kernel<<<H, 1024, 0, s>>>(rel.bias, static_cast<T*>(dtable), B, H, q_tiles, k_tiles, warps, causal ? 1 : 0, inv)
+  rel_table_grad_kernel<<<dim3(kGradCtas, H), kGradWarps * 32, 0, s>>>(rel.bias, static_cast<T*>(dtable), B, H, q_tiles, k_tiles, warps, causal ? 1 : 0, inv)
   if (table_dtype == FO_F32) FO_TABLE_GRAD(float);
   else if (table_dtype == FO_BF16) FO_TABLE_GRAD(__nv_bfloat16);
   else FO_TABLE_GRAD(__half);

@@ -121,12 +121,12 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       }
       if constexpr (rel_bias) {
         const int d0 = -static_cast<int>(row) - q_off;  // relative position of key 0
-        bias_first = rel_value(prm.rel, h, d0);
-        bias_last = rel_value(prm.rel, h, d0 + vis0 - 1);
+        bias_first = rel_value(prm.rel, h, d0) * prm.scale_log2;
+        bias_last = rel_value(prm.rel, h, d0 + vis0 - 1) * prm.scale_log2;
         if (prm.rel.vec != nullptr) {
           const float* const v = prm.rel.vec + rel_vec_row(prm.rel, b, h) * prm.rel.vec_width;
-          bias_first += __ldg(v);
-          bias_last += __ldg(v + vis0 - 1);
+          bias_first += __ldg(v) * prm.scale_log2;
+          bias_last += __ldg(v + vis0 - 1) * prm.scale_log2;
         }
       }
     }
@@ -232,10 +232,10 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const uint32_t drop_row = prm.ex.drop_base +
                               static_cast<uint32_t>(bh) * static_cast<uint32_t>(prm.Sq) * static_cast<uint32_t>(prm.Sk) +
                               static_cast<uint32_t>(row) * static_cast<uint32_t>(prm.Sk);
-    // The scores are scaled when the bias is added, not in the exponent; but away from the diagonal a
-    // relative bias is a constant, and without a vector bias beside it nothing is added to the scores
-    // there: they are scaled in the exponent, and the constant joins the reference maximum.
-    float exp_scale = 1.f, exp_add = 0.f;
+    // The scores are scaled when the bias is added, not in the exponent.  A relative bias is added to the
+    // unscaled scores, and away from the diagonal, where it is a constant, joins the reference maximum.
+    const float exp_scale = rel_bias ? prm.scale_log2 : 1.f;
+    float exp_add = 0.f;
     // a row-independent bias goes through shared memory, fetched one 128-key tile ahead
     const uint8_t* bias_vec = nullptr;
     float* sb = s_bias + s * 256;
@@ -337,21 +337,18 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       const bool need_mask = (k0n + kStepN > prm.Sk) || (prm.causal && k0n + kStepN - 1 > q0 + q_off);
       // relative positions of the warp's 32 rows and the step's keys: d_last - 94 to d_last
       const int d_last = k0n + kStepN - 1 - warp_row;
-      const int half = (tn & 1) ^ first;  // of the key tile
-      const bool step_vec = rel_vec && k0n < vec_last && k0n >= vec_first;
+      const float* step_vec = nullptr;
+      if (rel_vec && k0n < vec_last && k0n >= vec_first) step_vec = sb + ((tn >> 1) & 1) * 128 + ((tn & 1) ^ first) * kStepN;
       const RelSide side = rel_bias ? rel_side(prm.rel, d_last - (kStepN + 30), d_last) : kRelNear;
-      if constexpr (rel_bias) {
-        exp_add = side == kRelLeft ? rel_left : side == kRelRight ? rel_right : 0.f;
-        exp_scale = step_vec || side == kRelNear ? 1.f : prm.scale_log2;
-      }
+      if constexpr (rel_bias)
+        exp_add = side == kRelNear ? 0.f : (side == kRelLeft ? rel_left : rel_right) * prm.scale_log2;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         tmem_ld_wait(sr[c]);
         if ((warp & 3) == 0 && tn > 0) trace_event(prm, s, tn - 1, c == 0 ? 1 : 4);  // loads in
         if constexpr (rel_bias) {
-          const float* const bv = sb + ((tn >> 1) & 1) * 128 + half * kStepN + c * 32;
-          add_rel_bias<false>(sr[c], prm.scale_log2, side == kRelNear, rel_row + ((k0n + c * 32) >> 2),
-                       step_vec ? reinterpret_cast<const float4*>(bv) : nullptr);
+          if (side == kRelNear) add_rel_bias<false>(sr[c], rel_row + ((k0n + c * 32) >> 2));
+          if (rel_vec && step_vec != nullptr) add_rel_bias<true>(sr[c], reinterpret_cast<const float4*>(step_vec + c * 32));
         } else if constexpr (vec_bias) {
           const float4* bv = reinterpret_cast<const float4*>(sb + ((tn >> 1) & 1) * 128 + ((tn & 1) ^ first) * kStepN + c * 32);
 #pragma unroll

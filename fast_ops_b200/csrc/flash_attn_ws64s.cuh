@@ -24,6 +24,8 @@
 // not return; the softmax code fits the 168 registers of the launch bound with 84 bytes of spills.
 #pragma once
 
+#include <type_traits>
+
 #include "flash_attn_common.cuh"
 #include "flash_attn_ws.cuh"
 #include "flash_attn_ws64.cuh"
@@ -174,7 +176,7 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     tmem_relinquish_alloc_permit();
   }
   if (rel_bias && tid == 0) {
-    RelHead head = {rel_value(prm.rel, h, -prm.rel.zero), rel_value(prm.rel, h, prm.rel.width), 0, 0, 0};
+    RelHead head = {rel_value(prm.rel, h, -prm.rel.zero) * prm.scale_log2, rel_value(prm.rel, h, prm.rel.width) * prm.scale_log2, 0, 0, 0};
     if constexpr (rel_vec) {
       head.vec_row = static_cast<int>(rel_vec_row(prm.rel, b, h));
       const int4 extent = __ldg(prm.rel.vec_extent + head.vec_row);
@@ -197,7 +199,8 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     const uint32_t tS_tile = tmem_base + Cfg::kColS + lane_base;
     const uint32_t tO = tmem_base + Cfg::kColO + lane_base;
     // a relative bias: see flash_attn_ws64r.cuh
-    float exp_scale = prm.scale_log2, exp_add = 0.f;
+    const float exp_scale = prm.scale_log2;
+    float exp_add = 0.f;
     float* const sb = reinterpret_cast<float*>(smem + Cfg::kOffBias);
     float* const s_rel = reinterpret_cast<float*>(smem + Cfg::kOffRelVector);
     int rel_x = 0;  // where this row's bias of key 0 would be in its copy of the vector
@@ -218,41 +221,58 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     uint32_t sr[2][32];  // scores of the current step
 
     auto issue_load = [&](int tn, int c) { tmem_ld32(tS_tile + (tn & 1) * kStepN + c * 32, sr[c]); };
-    // Waits for those loads and applies the masks in place.
+    // Waits for those loads and applies masks and bias in place.
     auto prep_loads = [&](int tn) {
       const int k0n = tn * kStepN;
       const bool need_mask = (k0n + kStepN > prm.Sk) || (prm.causal && k0n + kStepN - 1 > q0 + q_off);
-      // relative positions of the warp's 32 rows and the step's keys: d_last - 94 to d_last
-      const int d_last = k0n + kStepN - 1 - (q0 + warp * 32 + q_off);
-      const bool step_vec = rel_vec && tn < rel_head->vec_last && tn >= rel_head->vec_first;
-      if constexpr (rel_vec) {
-        // Behind the barrier no thread reads the values of the step before (without one here there are none),
-        // whose buffer the next step's go to.
-        if (step_vec) {
-          cp_async_wait_all();
-          named_barrier_sync(1, 128);
-        }
-        fetch_vec(tn + 1);
-      }
-      const RelSide side = rel_bias ? rel_side(prm.rel, d_last - (kStepN + 30), d_last) : kRelNear;
+      bool near = false, step_vec = false;
       if constexpr (rel_bias) {
-        exp_add = side == kRelNear ? 0.f : side == kRelLeft ? rel_head->left : rel_head->right;
-        exp_scale = step_vec || side == kRelNear ? 1.f : prm.scale_log2;
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        tmem_ld_wait(sr[c]);
-        if constexpr (rel_bias)
-          add_rel_bias<true>(sr[c], prm.scale_log2, side == kRelNear,
-                             reinterpret_cast<const float4*>(s_rel + (rel_x + k0n + c * 32)), step_vec ? reinterpret_cast<const float4*>(sb + (tn & 1) * kStepN + c * 32) : nullptr);
-        if (need_mask) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int col = k0n + c * 32 + i;
-            if (col >= prm.Sk || (prm.causal && col > row + q_off)) sr[c][i] = 0xff800000u;  // -inf
+        // relative positions of the warp's 32 rows and the step's keys: d_last - 94 to d_last
+        const int d_last = k0n + kStepN - 1 - (q0 + warp * 32 + q_off);
+        const RelSide side = rel_side(prm.rel, d_last - (kStepN + 30), d_last);
+        near = side == kRelNear;
+        exp_add = near ? 0.f : side == kRelLeft ? rel_head->left : rel_head->right;
+        if constexpr (rel_vec) {
+          // Behind the barrier no thread reads the values of the step before (without one here there are none),
+          // whose buffer the next step's go to.
+          step_vec = tn < rel_head->vec_last && tn >= rel_head->vec_first;
+          if (step_vec) {
+            cp_async_wait_all();
+            named_barrier_sync(1, 128);
           }
+          fetch_vec(tn + 1);
         }
       }
+      auto mask = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const int col = k0n + c * 32 + i;
+          if (col >= prm.Sk || (prm.causal && col > row + q_off)) sr[c][i] = 0xff800000u;  // -inf
+        }
+      };
+      auto apply = [&]() {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if constexpr (rel_bias) {
+            if (near) add_rel_bias<true>(sr[c], reinterpret_cast<const float4*>(s_rel + (rel_x + k0n + c * 32)));
+            if (rel_vec && step_vec)
+              add_rel_bias<true>(sr[c], reinterpret_cast<const float4*>(sb + (tn & 1) * kStepN + c * 32));
+          }
+          if (need_mask) mask(c);
+        }
+      };
+      if constexpr (!rel_bias) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          tmem_ld_wait(sr[c]);
+          if (need_mask) mask(c);
+        }
+        return;
+      }
+      tmem_ld_wait(sr[0]);
+      tmem_ld_wait(sr[1]);
+      // one branch for all that few steps need (a branch for each: 235 us instead of 226 at B2 H16 S4096 D64)
+      if (near || step_vec || need_mask) apply();
     };
 
     if constexpr (rel_bias) {  // every thread's part of the vector is there

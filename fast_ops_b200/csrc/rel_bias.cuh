@@ -5,14 +5,15 @@
 // two-sided, n = |j - i - offset|, and the keys behind the query have a second set of buckets.
 //
 // The tile kernels read the bias of a head as a vector over the relative position d = j - i - offset, at
-// x = d + zero, times log2(e).  It is constant from -far_left down and from far_right up, so that only the
+// x = d + zero, divided by the softmax scale: it is added to Q K^T, and the scale in the exponent applies to both.
+// It is constant from -far_left down and from far_right up, so that only the
 // tiles near the diagonal read it at all; its ends reach kRelMargin further, which is more than a warp's
 // part of such a tile can.  A thread reads neighbouring values from a place of its own, 16 bytes at a time:
 // the vector is there four times, copy s shifted by s values, so that one of them is aligned for it
 // (64 values by 16 loads instead of 64).  The copies are 8 banks apart, so that from shared memory eight
 // threads read 32 banks.
 //
-// A vector bias beside it (key padding, as a rule) is brought into fp32 times log2(e) too, one row for each
+// A vector bias beside it (key padding, as a rule) is brought into the same form, one row for each
 // batch and head that has its own, with what lets the kernels pass over most of it: the end of the keys that
 // are not masked, behind which nothing is computed, and the 64-key steps from the first value that is not 0 to
 // the last one before that end.
@@ -42,12 +43,12 @@ __device__ __forceinline__ int rel_bucket(const RelBuckets& bk, int d) {
   return bk.two_sided && d > 0 ? lo + bk.n : lo;
 }
 
-// A bias in the units of the exponent, log2(e) * value, where -1e6 and less masks as -inf does.  (Taken as a
-// number, a mask that leaves a row without keys would give it an LSE of that size, from which the backward
+// A bias times `factor` (log2(e), or 1 / scale), where -1e6 and less masks as -inf does.  (Taken as a number,
+// a mask that leaves a row without keys would give it an LSE of that size, from which the backward
 // cannot tell P: at -1e9 the spacing of fp32 is 64, and P = exp(s - LSE) could be anything, infinity
 // included.  Rows with a key left do not change: e^-1e6 is 0.)
-__device__ __forceinline__ float scaled_or_masked(float v) {
-  return v <= -1e6f ? __int_as_float(0xff800000) : v * 1.4426950408889634f;
+__device__ __forceinline__ float scaled_or_masked(float v, float factor) {
+  return v <= -1e6f ? __int_as_float(0xff800000) : v * factor;
 }
 
 // What the tile kernels need; null `values`: no relative bias.
@@ -75,7 +76,7 @@ __device__ __forceinline__ RelSide rel_side(const RelBias& rel, int first, int l
   return last <= -rel.far_left ? kRelLeft : first >= rel.far_right ? kRelRight : kRelNear;
 }
 
-// Bias (times log2(e)) of relative position d for head h, whatever d is.
+// Bias (divided by the softmax scale) of relative position d for head h, whatever d is.
 __device__ __forceinline__ float rel_value(const RelBias& rel, int h, int d) {
   const int x = min(max(d, -rel.zero), rel.width - 1 - rel.zero) + rel.zero;
   return __ldg(rel.values + static_cast<int64_t>(h) * 4 * rel.stride + x);
@@ -93,32 +94,18 @@ __device__ __forceinline__ int rel_keys(const RelBias& rel, int b, int h, int ke
 // Keys of a row of `vec`: whole key tiles.
 __host__ __device__ inline int rel_vec_width(int Sk) { return (Sk + 127) / 128 * 128; }
 
-// Scales 32 scores and adds the bias where it is not the same for all of them: the relative bias near the
-// diagonal (`near`, this thread's values at `rel`, in shared memory or not), the vector bias where it is not zero
-// (`vec`, in shared memory, or null).
+// Adds 32 values of a bias, in shared memory or not, to 32 scores that are still to be scaled.
 template <bool kShared>
-__device__ __forceinline__ void add_rel_bias(uint32_t (&s)[32], float scale, bool near, const float4* rel, const float4* vec) {
-  auto add = [&](int i, float2 bias) {
-    const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(scale, scale), bias);
-    s[i] = __float_as_uint(x.x);
-    s[i + 1] = __float_as_uint(x.y);
-  };
-  if (near) {
+__device__ __forceinline__ void add_rel_bias(uint32_t (&s)[32], const float4* bias) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 r = kShared ? rel[i] : __ldg(rel + i);
-      add(4 * i, make_float2(r.x, r.y));
-      add(4 * i + 2, make_float2(r.z, r.w));
-    }
-    scale = 1.f;
-  }
-  if (vec != nullptr) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float4 v = vec[i];
-      add(4 * i, make_float2(v.x, v.y));
-      add(4 * i + 2, make_float2(v.z, v.w));
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float4 r = kShared ? bias[i] : __ldg(bias + i);
+    const float2 lo = __fadd2_rn(make_float2(__uint_as_float(s[4 * i]), __uint_as_float(s[4 * i + 1])), make_float2(r.x, r.y));
+    const float2 hi = __fadd2_rn(make_float2(__uint_as_float(s[4 * i + 2]), __uint_as_float(s[4 * i + 3])), make_float2(r.z, r.w));
+    s[4 * i] = __float_as_uint(lo.x);
+    s[4 * i + 1] = __float_as_uint(lo.y);
+    s[4 * i + 2] = __float_as_uint(hi.x);
+    s[4 * i + 3] = __float_as_uint(hi.y);
   }
 }
 
