@@ -182,21 +182,33 @@ __device__ __forceinline__ void load_bias_rows32(const AttnExtras& ex, const uin
   }
 }
 
-// Adds a warp's sums, one per lane, to the buckets of their relative positions `d`.  Lanes of one bucket
-// are neighbours (d ascends with the lane, or is the same in all): each run is summed into its first lane,
-// which adds it to the accumulator.  The accumulator belongs to this warp alone, so the order of the
-// additions does not change from run to run.
-__device__ __forceinline__ void add_diagonals(const RelBias& rel, float* acc, int d, int lane, float sum) {
-  const int bucket = __ldg(rel.bucket_of + d + rel.zero);
+// Adds a warp's sums along diagonals to the buckets of their relative positions: sums[k] of lane l belongs to
+// bucket[k], relative position ascending with l and descending with k.  Lanes of one bucket are neighbours: each
+// run is summed into its first lane, which adds it to the accumulator.  The accumulator belongs to this warp alone,
+// so the order of the additions does not change from run to run.
+template <int kN>
+__device__ __forceinline__ void add_diagonals(float* acc, const int (&bucket)[kN], int lane, float (&sums)[kN]) {
+  uint32_t heads[kN];  // lanes that begin a run
+  int end[kN];         // lane behind this lane's run
 #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const float v = __shfl_down_sync(0xffffffffu, sum, off);
-    const int other = __shfl_down_sync(0xffffffffu, bucket, off);
-    if (lane + off < 32 && other == bucket) sum += v;
+  for (int k = 0; k < kN; ++k) {
+    const int before = __shfl_up_sync(0xffffffffu, bucket[k], 1);
+    heads[k] = __ballot_sync(0xffffffffu, lane == 0 || before != bucket[k]);
+    const uint32_t above = heads[k] & (0xfffffffeu << lane);
+    end[k] = above ? __ffs(above) - 1 : 32;
   }
-  const int before = __shfl_up_sync(0xffffffffu, bucket, 1);
-  if (lane == 0 || before != bucket) atomicAdd(acc + bucket, sum);
-  __syncwarp();
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1)
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      const float v = __shfl_down_sync(0xffffffffu, sums[k], off);
+      sums[k] += lane + off < end[k] ? v : 0.f;
+    }
+#pragma unroll
+  for (int k = 0; k < kN; ++k) {
+    if (heads[k] >> lane & 1u) atomicAdd(acc + bucket[k], sums[k]);
+    __syncwarp();
+  }
 }
 
 // grid = (key tiles, B*H); block = BwdConfig<D, kExt>::kThreads.
@@ -376,7 +388,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       // relative positions of the warp's 32 keys and its query columns: d_first to d_first + 30 + kCols
       const int d_first = warp_key - (qc0 + kCols - 1);
       const RelSide side = rel_bias ? rel_side(prm.rel, d_first, d_first + 30 + kCols) : kRelNear;
-      const bool rel_near = side == kRelNear;
+      const bool rel_near = rel_bias && side == kRelNear;
+      // buckets of the diagonals that this lane will hold the sums of, fetched ahead
+      int diag_bucket[kPieces + 1] = {};
+      if (rel_near && rel_acc != nullptr) {
+#pragma unroll
+        for (int k = 0; k <= kPieces; ++k)
+          diag_bucket[k] = __ldg(prm.rel.bucket_of + (prm.rel.zero + d_first + kCols - 1 + lane - 32 * k));
+      }
       // What does not depend on S^T comes first: the keep decisions and the first bias values.
       uint32_t keep[kPieces];  // dropout: bit x of keep[cc] = element kept
       if constexpr (has_drop) {
@@ -546,8 +565,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                   const float v = __shfl_sync(0xffffffffu, dsv[y], (lane + x + y) & 31);
-                  if (lane + x + y < 32) diag[cc] += v;
-                  else diag[cc + 1] += v;
+                  const bool first = lane + x + y < 32;
+                  diag[cc] += first ? v : 0.f;
+                  diag[cc + 1] += first ? 0.f : v;
                 }
               } else if constexpr (rel_bias) {
                 far_sum = __fadd2_rn(far_sum, __fadd2_rn(make_float2(dsv[0], dsv[1]), make_float2(dsv[2], dsv[3])));
@@ -577,10 +597,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
             float ds_sum = far_sum.x + far_sum.y;
             if (diag_sums) {
 #pragma unroll
-              for (int k = 0; k <= kPieces; ++k) {
-                ds_sum += diag[k];
-                add_diagonals(prm.rel, rel_acc, d_first + kCols - 1 + lane - 32 * k, lane, diag[k]);
-              }
+              for (int k = 0; k <= kPieces; ++k) ds_sum += diag[k];
+              add_diagonals<kPieces + 1>(rel_acc, diag_bucket, lane, diag);
             }
             // both sums over the warp: the lower half of the lanes goes on with dS, the upper with P
             float sum = lane < 16 ? ds_sum : p_sum;

@@ -258,7 +258,8 @@ int64_t expanded_bytes(const RelBias& bias, int H, int64_t bias_rows, int Sk) {
   return (static_cast<int64_t>(H) * 4 * bias.stride + bias_rows * width + bias.stride) * 4 + bias_rows * 16;
 }
 
-int set_expanded(RelArgs* rel, void* workspace, const fo::AttnExtras& ex, int B, int H, int Sk) {
+int set_expanded(RelArgs* rel, void* workspace, const fo::AttnExtras& ex, int B, int H, int Sk, bool needed) {
+  if (!needed) return FO_OK;
   FO_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be given, 16-byte aligned");
   FO_REQUIRE(B > 0 && H > 0, "B and H must be positive (got %d %d)", B, H);
   RelBias& bias = rel->bias;
@@ -445,7 +446,8 @@ extern "C" int fo_rel_attn_fwd(const void* q, const void* k, const void* v, void
   if (int rc = check_bias_strides(bias, bias_strides)) return rc;
   fo::AttnExtras ex;
   if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset)) return rc;
-  if (int rc = set_expanded(&rel, workspace, ex, B, H, Sk)) return rc;
+  // one query row without an LSE: the decoding kernel finds the buckets by itself
+  if (int rc = set_expanded(&rel, workspace, ex, B, H, Sk, Sq > 1 || lse != nullptr || ex.dropout)) return rc;
   return fo::attn_fwd_impl(q, k, v, o, lse, B, H, Sq, Sk, D, q_strides, k_strides, v_strides, o_strides, dtype, causal,
                            softmax_scale, &ex, &rel, device, stream);
 }
@@ -473,7 +475,7 @@ extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, cons
   if (int rc = check_bias_strides(bias, bias_strides)) return rc;
   fo::AttnExtras ex;
   if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset)) return rc;
-  if (int rc = set_expanded(&rel, const_cast<void*>(workspace), ex, B, H, Sk)) return rc;
+  if (int rc = set_expanded(&rel, const_cast<void*>(workspace), ex, B, H, Sk, true)) return rc;
   if (dtable != nullptr) {
     rel.bias.tile_sums = reinterpret_cast<float2*>(partials);
     rel.bias.acc = partials + tile_sum_floats(B, H, Sq, Sk, D, ex.dropout != 0);

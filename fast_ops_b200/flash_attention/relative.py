@@ -71,77 +71,90 @@ def _workspace_bytes(H: int, M: int, N: int, num_buckets: int, max_distance: int
     return size
 
 
+@lru_cache(maxsize=256)
+def _partial_floats(B: int, H: int, M: int, N: int, D: int, num_buckets: int, dropout: bool) -> int:
+    size = _lib.load().fo_rel_attn_bwd_workspace(B, H, M, N, D, num_buckets, int(dropout))
+    _lib.check(-1 if size < 0 else 0)
+    return size // 4
+
+
 class _Call:
     """The checked arguments of one call, shared by forward and backward."""
 
     def __init__(self, Q: Tensor, K: Tensor, V: Tensor, table: Tensor, max_distance: int, bidirectional: bool,
                  query_offset: int, causal: bool, softmax_scale: Optional[float], dropout_p: float,
                  rng: Optional[Tuple[int, int]]):
-        if not all(isinstance(t, Tensor) for t in (Q, K, V, table)):
+        if not (isinstance(Q, Tensor) and isinstance(K, Tensor) and isinstance(V, Tensor) and isinstance(table, Tensor)):
             raise RuntimeError("Q, K, V and table must be tensors")
-        if Q.dim() != 4 or K.dim() != 4 or V.dim() != 4:
+        q_shape, k_shape, table_shape = Q.shape, K.shape, table.shape
+        if len(q_shape) != 4 or len(k_shape) != 4:
             raise RuntimeError("Q, K, V must be 4-D")
-        if not Q.is_cuda:
+        index = Q.get_device()
+        if index < 0:
             raise RuntimeError("fast_ops_b200 attention needs CUDA tensors (there is no CPU path)")
-        if any(t.device != Q.device for t in (K, V, table)):
+        if K.get_device() != index or V.get_device() != index or table.get_device() != index:
             raise RuntimeError("Q, K, V and table must be on the same device")
-        code = _CODES.get(Q.dtype)
+        dtype = Q.dtype
+        code = _CODES.get(dtype)
         if code is None:
-            raise RuntimeError(f"inputs must be float16 or bfloat16, got {Q.dtype}")
-        if K.dtype != Q.dtype or V.dtype != Q.dtype:
+            raise RuntimeError(f"inputs must be float16 or bfloat16, got {dtype}")
+        if K.dtype != dtype or V.dtype != dtype:
             raise RuntimeError("Q, K, V must have the same dtype")
-        if table.dtype not in (Q.dtype, torch.float32):
+        table_code = code if table.dtype == dtype else _lib.FO_F32
+        if table_code != code and table.dtype != torch.float32:
             raise RuntimeError(f"table must be float32 or have Q's dtype, got {table.dtype}")
-        B, H, M, D = Q.shape
-        if K.shape[:2] != (B, H) or K.shape[3] != D or V.shape != K.shape:
-            raise RuntimeError(f"shape mismatch: Q {tuple(Q.shape)}, K {tuple(K.shape)}, V {tuple(V.shape)}")
-        if table.dim() != 2 or table.shape[1] != H:
-            raise RuntimeError(f"table must be (num_buckets, {H}), got {tuple(table.shape)}")
+        B, H, M, D = q_shape
+        if k_shape[0] != B or k_shape[1] != H or k_shape[3] != D or V.shape != k_shape:
+            raise RuntimeError(f"shape mismatch: Q {tuple(q_shape)}, K {tuple(k_shape)}, V {tuple(V.shape)}")
+        if len(table_shape) != 2 or table_shape[1] != H:
+            raise RuntimeError(f"table must be (num_buckets, {H}), got {tuple(table_shape)}")
         if D > 128 or D % 8 != 0 or D == 0:
             raise RuntimeError(f"head_dim must be a multiple of 8 and <= 128, got {D}")
-        for name, t in (("Q", Q), ("K", K), ("V", V)):
-            if t.stride(3) != 1:
-                raise RuntimeError(f"{name}: the last dimension must be contiguous")
+        if Q.stride(3) != 1 or K.stride(3) != 1 or V.stride(3) != 1:
+            raise RuntimeError("Q, K, V: the last dimension must be contiguous")
         if not 0.0 <= dropout_p < 1.0:
             raise RuntimeError(f"dropout_p must be in [0, 1), got {dropout_p}")
         if not 0 <= query_offset <= 2**29:
             raise RuntimeError(f"query_offset must be in [0, 2^29], got {query_offset}")
-        self.B, self.H, self.M, self.D, self.N = B, H, M, D, K.shape[2]
-        self.code, self.device, self.index = code, Q.device, Q.get_device()
-        self.table_dtype = _lib.FO_F32 if table.dtype == torch.float32 else code
-        self.num_buckets = table.shape[0]
-        self.key = (self.num_buckets, int(max_distance), bool(bidirectional))
-        self.starts, self.n_starts = _starts_array(*self.key)
-        self.bidirectional, self.offset, self.causal = int(bool(bidirectional)), int(query_offset), int(bool(causal))
-        self.scale = float(softmax_scale) if softmax_scale is not None else 1.0 / math.sqrt(D)
+        self.B, self.H, self.M, self.D, self.N = B, H, M, D, k_shape[2]
+        self.code, self.device, self.index, self.table_code = code, Q.device, index, table_code
+        self.num_buckets = table_shape[0]
+        self.key = key = (self.num_buckets, int(max_distance), bool(bidirectional))
+        self.starts, self.n_starts = _starts_array(*key)
+        self.bidirectional, self.offset, self.causal = int(key[2]), int(query_offset), 1 if causal else 0
+        self.scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
         self.dropout_p = float(dropout_p)
-        if self.dropout_p > 0.0 and rng is None:
+        if rng is not None:
+            rng = (rng[0] & (2**64 - 1), rng[1] & (2**64 - 1))
+        elif self.dropout_p > 0.0:
             rng = next_dropout_rng(Q.device, B * H * M * self.N)
-        self.rng = (0, 0) if rng is None else (rng[0] & (2**64 - 1), rng[1] & (2**64 - 1))
+        self.rng = rng or (0, 0)
 
     def bias(self, bias: Optional[Tensor], Q: Tensor):
-        if bias is not None and bias.dim() == 4 and bias.shape[2] != 1:
+        if bias is None:
+            return None, 0, (None, None, _lib.FO_F32)
+        if bias.dim() == 4 and bias.shape[2] != 1:
             raise RuntimeError("beside a relative bias, bias must be (1 or B, 1 or H, 1, N): the same for every query")
         kept, ptr, strides, code = _prepare_bias(bias, Q, self.B, self.H, self.M, self.N)
-        rows = 0
-        if strides is not None:
-            strides[2] = 0  # a single query row's stride says nothing
-            rows = (self.B if strides[0] else 1) * (self.H if strides[1] else 1)
+        strides[2] = 0  # a single query row's stride says nothing
+        rows = (self.B if strides[0] else 1) * (self.H if strides[1] else 1)
         return kept, rows, (ptr, strides, code)
 
     def forward(self, Q: Tensor, K: Tensor, V: Tensor, table: Tensor, bias: Optional[Tensor], lse: bool):
-        """(O, LSE or None, the expanded bias)."""
+        """(O, LSE or None, the expanded bias or None where nothing reads it)."""
         O = torch.empty_like(Q, memory_format=torch.contiguous_format)
         lse_t = Q.new_empty((self.B, self.H, self.M), dtype=torch.float32) if lse else None
         kept, rows, bias_args = self.bias(bias, Q)
-        workspace = torch.empty(_workspace_bytes(self.H, self.M, self.N, *self.key, self.offset, rows),
-                                dtype=torch.uint8, device=self.device)
+        workspace = None
+        if lse or self.M > 1 or self.dropout_p > 0.0:
+            workspace = torch.empty(_workspace_bytes(self.H, self.M, self.N, *self.key, self.offset, rows),
+                                    dtype=torch.uint8, device=self.device)
         ts = table.stride()
         _lib.check(_lib.load().fo_rel_attn_fwd(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), lse_t.data_ptr() if lse else None, self.B, self.H, self.M, self.N, self.D,
             _strides3(Q), _strides3(K), _strides3(V), _strides3(O), self.code, self.causal, self.scale,
-            table.data_ptr(), _I64x2(ts[0], ts[1]), self.table_dtype, self.starts, self.n_starts, self.bidirectional,
-            self.offset, workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
+            table.data_ptr(), _I64x2(ts[0], ts[1]), self.table_code, self.starts, self.n_starts, self.bidirectional,
+            self.offset, None if workspace is None else workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
             _lib.current_stream_ptr(self.index)))
         return O, lse_t, workspace
 
@@ -164,8 +177,7 @@ class _Call:
         dtable = None
         if table_grad is not None:
             dtable = torch.empty((self.num_buckets, self.H), dtype=table_grad, device=self.device)
-            partials = lib.fo_rel_attn_bwd_workspace(self.B, self.H, self.M, self.N, self.D, self.num_buckets,
-                                                     int(self.dropout_p > 0.0)) // 4
+            partials = _partial_floats(self.B, self.H, self.M, self.N, self.D, self.num_buckets, self.dropout_p > 0.0)
         # one scratch block: the fp32 dQ accumulator (B, H, M, D), the table's partial sums, rowsum(O o dO) (B, H, M)
         scratch = torch.empty(rows * (self.D + 1) + partials, dtype=torch.float32, device=self.device)
         dq_accum = scratch.data_ptr()
@@ -177,7 +189,7 @@ class _Call:
             partial_sums + 4 * partials, partial_sums,
             self.B, self.H, self.M, self.N, self.D,
             _strides3(Q), _strides3(K), _strides3(V), _strides3(O), _strides3(dO), _strides3(dQ), _strides3(dK),
-            _strides3(dV), self.code, self.causal, self.scale, self.table_dtype, self.starts, self.n_starts,
+            _strides3(dV), self.code, self.causal, self.scale, self.table_code, self.starts, self.n_starts,
             self.bidirectional, self.offset, workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
             _lib.current_stream_ptr(self.index)))
         return dQ, dK, dV, dtable

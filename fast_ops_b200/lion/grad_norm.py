@@ -7,6 +7,7 @@ rewritten and nothing waits for the host.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Iterable, List, Optional, Tuple
 
 import torch
@@ -29,29 +30,42 @@ def is_dense(t: Tensor) -> bool:
     return True
 
 
+_CODES = {torch.float16: _lib.FO_F16, torch.bfloat16: _lib.FO_BF16, torch.float32: _lib.FO_F32}
+
+
+@lru_cache(maxsize=64)
+def _workspace_doubles(n: int) -> int:
+    return int(_lib.load().fo_grad_norm_workspace(n))
+
+
 class GradList:
-    """ctypes image of the gradients of one norm call."""
+    """ctypes image of the gradients of one norm call.  Checks and pointers are gathered column by
+    column: at a few hundred tensors the attribute accesses are what the call costs the host."""
 
     def __init__(self, grads: List[Tensor]):
         if not grads:
             raise RuntimeError("grad_norm needs at least one tensor")
-        for g in grads:
-            if not isinstance(g, Tensor) or g.layout != torch.strided:
-                raise RuntimeError("gradients must be dense tensors")
-            if not g.is_cuda:
+        try:
+            devices = {g.get_device() for g in grads}
+            codes = [_CODES.get(g.dtype) for g in grads]
+            if min(devices) < 0:
                 raise RuntimeError("fast_ops_b200 grad_norm needs CUDA tensors (there is no CPU path)")
-        device = grads[0].device
-        for g in grads:
-            if g.device != device:
+            if len(devices) > 1:
                 raise RuntimeError("all gradients must be on one device")
-            if not is_dense(g):
+            if None in codes:
+                raise RuntimeError(f"unsupported dtype {grads[codes.index(None)].dtype}")
+            if not all([g.is_contiguous() for g in grads]) and not all([is_dense(g) for g in grads]):
                 raise RuntimeError("expected tensor to be contiguous")
+            ptrs = [g.data_ptr() for g in grads]  # a sparse tensor has none and raises RuntimeError
+            numels = [g.numel() for g in grads]
+        except AttributeError:
+            raise RuntimeError("gradients must be tensors") from None
         n = len(grads)
-        self.n, self.device, self.device_index = n, device, device.index
-        self.ptrs = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
-        self.numels = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
-        self.dtypes = (ctypes.c_int * n)(*[_lib.dtype_code(g.dtype) for g in grads])
-        self.doubles = int(_lib.load().fo_grad_norm_workspace(n))
+        self.n, self.device, self.device_index = n, grads[0].device, devices.pop()
+        self.ptrs = (ctypes.c_void_p * n)(*ptrs)
+        self.numels = (ctypes.c_int64 * n)(*numels)
+        self.dtypes = (ctypes.c_int * n)(*codes)
+        self.doubles = _workspace_doubles(n)
 
     def launch(self, max_norm: float, sumsq: Optional[Tensor] = None) -> Tensor:
         """(norm, clipping factor) as two floats on the device; `sumsq`, if given, receives the sum of

@@ -133,9 +133,7 @@ class Lion(Optimizer):
         self._momentum_dtype = momentum_dtype
         self._lists: Dict[int, tuple] = {}  # group index -> (address signature, prepared launches)
         self.max_grad_norm = max_grad_norm
-        #: 0-d fp32 tensor: the norm of all gradients at the latest step, before clipping; None before the
-        #: first one and without max_grad_norm
-        self.grad_norm: Optional[Tensor] = None
+        self._norm_coef: Optional[Tensor] = None  # (norm, clipping factor) of the latest step
         self._grad_list: Optional[Tuple[list, Optional[GradList]]] = None
         self._pg = process_group
         self._zero = None
@@ -186,7 +184,12 @@ class Lion(Optimizer):
             self._zero.step()
             return
         lib = _lib.load()
-        clip = self._clip_factor() if self.max_grad_norm is not None else None
+        clip = None
+        if self.max_grad_norm is not None:
+            self._norm_coef = self._launch_norm()
+            if self._norm_coef is None:
+                return  # no parameter has a gradient
+            clip = self._norm_coef.data_ptr() + 4
         for gi, group in enumerate(self.param_groups):
             lr = float(group["lr"])
             weight_decay = float(group["weight_decay"])
@@ -199,7 +202,7 @@ class Lion(Optimizer):
                 if clip is None:
                     _lib.check(lib.fo_lion_multi_tensor_step(*args, *where))
                 else:
-                    _lib.check(lib.fo_lion_multi_tensor_step_clipped(*args, clip.data_ptr(), *where))
+                    _lib.check(lib.fo_lion_multi_tensor_step_clipped(*args, clip, *where))
 
     def _group_lists(self, gi: int, group) -> list:
         """The group's prepared launches.  A training loop presents the same tensors step after step:
@@ -212,24 +215,29 @@ class Lion(Optimizer):
             self._lists[gi] = cached
         return cached[1]
 
-    def _clip_factor(self) -> Optional[Tensor]:
-        """Launches the norm over the gradients of all groups; returns the clipping factor, a device
-        float, or None when no parameter has a gradient."""
-        max_norm = float(self.max_grad_norm)
-        if not max_norm > 0:
-            raise RuntimeError(f"max_grad_norm must be positive, got {max_norm}")
+    @property
+    def grad_norm(self) -> Optional[Tensor]:
+        """The norm of all gradients at the latest step, before clipping: a 0-d fp32 tensor.  None before
+        the first step, without `max_grad_norm`, and after a step in which no parameter had a gradient."""
+        return None if self._norm_coef is None else self._norm_coef[0]
+
+    def _launch_norm(self) -> Optional[Tensor]:
+        """Launches the norm over the gradients of all groups; returns (norm, clipping factor) on the
+        device, or None when no parameter has a gradient."""
+        max_norm = self._checked_max_norm()
         lists = [tl for gi, group in enumerate(self.param_groups) for tl in self._group_lists(gi, group)]
         if self._grad_list is None or len(self._grad_list[0]) != len(lists) or any(
                 a is not b for a, b in zip(self._grad_list[0], lists)):
             grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
             self._grad_list = (lists, GradList(grads) if grads else None)
         grad_list = self._grad_list[1]
-        if grad_list is None:
-            self.grad_norm = None
-            return None
-        result = grad_list.launch(max_norm)
-        self.grad_norm = result[0]
-        return result[1]
+        return None if grad_list is None else grad_list.launch(max_norm)
+
+    def _checked_max_norm(self) -> float:
+        max_norm = float(self.max_grad_norm)
+        if not max_norm > 0:
+            raise RuntimeError(f"max_grad_norm must be positive, got {max_norm}")
+        return max_norm
 
     def load_state_dict(self, state_dict) -> None:
         """As torch.optim.Optimizer.load_state_dict; in process_group mode the loaded momentum
@@ -344,14 +352,12 @@ class _Zero1State:
         gradient lies in one slice), then the factor: the same on all ranks."""
         import torch.distributed as dist
 
-        max_norm = float(self.opt.max_grad_norm)
-        if not max_norm > 0:
-            raise RuntimeError(f"max_grad_norm must be positive, got {max_norm}")
+        max_norm = self.opt._checked_max_norm()
         sumsq = self.sumsq_fn(self.flat_g, self.begin, self.end)
         if self.world > 1:
             dist.all_reduce(sumsq, group=self.group)
         result = self.finish_norm_fn(sumsq, max_norm)
-        self.opt.grad_norm = result[0]
+        self.opt._norm_coef = result
         return result[1]
 
     @torch.no_grad()

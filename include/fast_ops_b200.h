@@ -169,7 +169,7 @@ int fo_flash_attn_bwd_ex(const void* q, const void* k, const void* v, const void
  *                whether dropout_p > 0; num_buckets: n_starts, twice that if two-sided).
  *
  * Sq = 1 without dropout runs in the decoding kernel, which fills the workspace only if
- * there is an lse (a backward may follow).
+ * there is an lse (a backward may follow); without one it may be NULL.
  * The workspace functions return -1 for arguments that the calls refuse.
  */
 int64_t fo_rel_attn_workspace(int H, int Sq, int Sk, const int* starts, int n_starts, int two_sided, int query_offset,
