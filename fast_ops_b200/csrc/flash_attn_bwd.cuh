@@ -490,18 +490,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       };
       exponentials();
       if (warp == 0) bwd_trace(prm, 0, it, 4);
-      float p_sum = 0.f;
-      if constexpr (rel_bias) {
-        if (rel_acc != nullptr) {
-          float2 p2 = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int cc = 0; cc < kPieces; ++cc)
-#pragma unroll
-            for (int x = 0; x < 32; x += 2)
-              p2 = __fadd2_rn(p2, make_float2(__uint_as_float(sr[cc][x]), __uint_as_float(sr[cc][x + 1])));
-          p_sum = p2.x + p2.y;
-        }
-      }
       // ---- P^T (zero where the forward dropped the element), 16-bit, over the first half of this thread's S^T columns ----
       uint32_t pp[kPieces * 16];
 #pragma unroll
@@ -521,6 +509,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       tcgen05_fence_before_sync();
       mbar_arrive(bar_p_full + Cfg::par(it));  // the dV matmul may start
       if (warp == 0) bwd_trace(prm, 0, it, 5);
+      float p_sum = 0.f;
+      if constexpr (rel_bias) {
+        if (rel_acc != nullptr) {
+          float2 p2 = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int cc = 0; cc < kPieces; ++cc)
+#pragma unroll
+            for (int x = 0; x < 32; x += 2)
+              p2 = __fadd2_rn(p2, make_float2(__uint_as_float(sr[cc][x]), __uint_as_float(sr[cc][x + 1])));
+          p_sum = p2.x + p2.y;
+        }
+      }
 
       // ---- dS^T = P^T o (dP^T - delta) * scale, dP = 0 for a dropped element ----
       mbar_wait(bar_delta_full + Cfg::par(it), Cfg::phase(it), cta_abort, dstat, FO_STATUS_TIMEOUT_TMA);
@@ -532,16 +532,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // query tile's dP^T matmul.
         uint8_t* const ds_tile = sDS + (it & (Cfg::kSlots - 1)) * Cfg::kDSBytes;
         uint32_t dd[kPieces * 16];
-        // Table gradient: the sum of dS over the part, and near the diagonal also along the diagonals of its
-        // 32-column pieces: the value of key row r and column x goes to lane (r - x) mod 32, where those
-        // with r >= x and those with r < x are two diagonals 32 apart.  diag[k]: relative position
-        // d_first + kCols - 1 + lane - 32 k.
-        const bool diag_sums = rel_bias && rel_near && rel_acc != nullptr;
-        float diag[kPieces + 1];
-        float2 far_sum = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k <= kPieces; ++k) diag[k] = 0.f;
-        auto ds_columns = [&](auto diagonals) {
+        auto ds_columns = [&]() {
 #pragma unroll
           for (int cc = 0; cc < kPieces; ++cc) {
             const float* nd = sNegDelta + (it & (Cfg::kSlots - 1)) * 128 + part * kCols + cc * 32;
@@ -561,28 +552,16 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
                 }
                 dsv[y] = __uint_as_float(sr[cc][x + y]) * fmaf(g, dp_scale, ndv[y]);
               }
-              if constexpr (diagonals.value) {
+              if constexpr (rel_bias) {
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                  const float v = __shfl_sync(0xffffffffu, dsv[y], (lane + x + y) & 31);
-                  const bool first = lane + x + y < 32;
-                  diag[cc] += first ? v : 0.f;
-                  diag[cc + 1] += first ? 0.f : v;
-                }
-              } else if constexpr (rel_bias) {
-                far_sum = __fadd2_rn(far_sum, __fadd2_rn(make_float2(dsv[0], dsv[1]), make_float2(dsv[2], dsv[3])));
+                for (int y = 0; y < 4; ++y) sr[cc][x + y] = __float_as_uint(dsv[y]);  // P is not needed any more
               }
               dd[cc * 16 + (x >> 1)] = pack2<kBf16>(dsv[0], dsv[1]);
               dd[cc * 16 + (x >> 1) + 1] = pack2<kBf16>(dsv[2], dsv[3]);
             }
           }
         };
-        if constexpr (rel_bias) {
-          if (diag_sums) ds_columns(std::true_type{});
-          else ds_columns(std::false_type{});
-        } else {
-          ds_columns(std::false_type{});
-        }
+        ds_columns();
         tmem_st_packed(tDP, dd);
 #pragma unroll
         for (int u = 0; u < kPieces * 4; ++u)
@@ -594,11 +573,41 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (warp == 0) bwd_trace(prm, 0, it, 1);
         if constexpr (rel_bias) {
           if (rel_acc != nullptr) {
-            float ds_sum = far_sum.x + far_sum.y;
-            if (diag_sums) {
+            // The table's gradient, behind the hand-over, while the tensor core works: the sum of dS over the part,
+            // and near the diagonal the sums along the diagonals.  Those are taken in pieces of 32 columns: the
+            // value of key row r and column x goes to lane (r - x) mod 32, where those with r >= x and those with
+            // r < x are two diagonals 32 apart.  diag[k]: relative position d_first + kCols - 1 + lane - 32 k.
+            float ds_sum = 0.f;
+            if (rel_near) {
+              float diag[kPieces + 1];
+#pragma unroll
+              for (int k = 0; k <= kPieces; ++k) diag[k] = 0.f;
+#pragma unroll
+              for (int cc = 0; cc < kPieces; ++cc) {
+#pragma unroll
+                for (int x = 0; x < 32; x += 8) {
+                  float v[8];
+#pragma unroll
+                  for (int y = 0; y < 8; ++y) v[y] = __shfl_sync(0xffffffffu, __uint_as_float(sr[cc][x + y]), (lane + x + y) & 31);
+#pragma unroll
+                  for (int y = 0; y < 8; ++y) {
+                    const bool first = lane + x + y < 32;
+                    diag[cc] += first ? v[y] : 0.f;
+                    diag[cc + 1] += first ? 0.f : v[y];
+                  }
+                }
+              }
 #pragma unroll
               for (int k = 0; k <= kPieces; ++k) ds_sum += diag[k];
               add_diagonals<kPieces + 1>(rel_acc, diag_bucket, lane, diag);
+            } else {
+              float2 sum2 = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int cc = 0; cc < kPieces; ++cc)
+#pragma unroll
+                for (int x = 0; x < 32; x += 2)
+                  sum2 = __fadd2_rn(sum2, make_float2(__uint_as_float(sr[cc][x]), __uint_as_float(sr[cc][x + 1])));
+              ds_sum = sum2.x + sum2.y;
             }
             // both sums over the warp: the lower half of the lanes goes on with dS, the upper with P
             float sum = lane < 16 ? ds_sum : p_sum;
