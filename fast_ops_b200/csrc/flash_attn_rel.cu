@@ -127,11 +127,11 @@ rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, i
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int parts = warps / 4, cols = fo::kBlockM / parts;  // four warps share a part's queries
   double left = 0, right = 0;
-  for (int64_t item = rank * kGradWarps + warp; item < static_cast<int64_t>(B) * n_q_tiles * parts; item += kGradCtas * kGradWarps) {
+  const uint32_t items = static_cast<uint32_t>(B) * n_q_tiles * parts;
+  for (uint32_t item = rank * kGradWarps + warp; item < items; item += kGradCtas * kGradWarps) {
     const int p = static_cast<int>(item % parts);
-    const int64_t bi = item / parts;
-    const int i = static_cast<int>(bi % n_q_tiles);
-    const int b = static_cast<int>(bi / n_q_tiles);
+    const uint32_t bi = item / parts;
+    const int b = static_cast<int>(bi / n_q_tiles), i = static_cast<int>(bi - static_cast<uint32_t>(b) * n_q_tiles);
     const float2* const row = rel.tile_sums + ((static_cast<int64_t>(b) * H + h) * n_q_tiles + i) * n_k_tiles * warps + p * 4;
     const int q_first = i * fo::kBlockM + p * cols + rel.offset;  // key position of the part's first query
     // key tiles that this query tile sees and that have keys (the backward visits no others)
@@ -174,16 +174,16 @@ rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, i
   }
   // rows of the sums by bucket: (batch, key tile, warp), of which this block takes every kGradCtas-th
   const int per_batch = n_k_tiles * warps;
-  const int64_t rows = static_cast<int64_t>(B) * per_batch;
+  const uint32_t rows = static_cast<uint32_t>(B) * per_batch;
   const int nb = rel.num_buckets;
   for (int u0 = 0; u0 < nb; u0 += 32) {
     const int u = u0 + lane;
     double sum = 0;
     if (u < nb) {
 #pragma unroll 8
-      for (int64_t r = rank * kGradWarps + warp; r < rows; r += kGradCtas * kGradWarps) {
-        const int64_t b = r / per_batch;
-        sum += static_cast<double>(rel.acc[((b * H + h) * per_batch + (r - b * per_batch)) * nb + u]);
+      for (uint32_t r = rank * kGradWarps + warp; r < rows; r += kGradCtas * kGradWarps) {
+        const uint32_t b = r / per_batch;  // row (b * H + h) * per_batch + r - b * per_batch
+        sum += static_cast<double>(rel.acc[(static_cast<int64_t>(b * (H - 1) + h) * per_batch + r) * nb + u]);
       }
     }
     part[warp][lane] = sum;
@@ -489,6 +489,7 @@ extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, cons
   FO_REQUIRE(guard.ok, "cannot make device %d current", device);
   const int q_tiles = (Sq + fo::kBlockM - 1) / fo::kBlockM, k_tiles = (Sk + fo::kBlockN - 1) / fo::kBlockN;
   const int warps = bwd_warps(D, ex.dropout != 0);
+  FO_REQUIRE(4LL * B * q_tiles < (1LL << 31) && 1LL * B * k_tiles * warps < (1LL << 31), "too many tiles for the table's gradient");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const float inv = 1.f / softmax_scale;
 #define FO_TABLE_GRAD(T)                                                                                             \
