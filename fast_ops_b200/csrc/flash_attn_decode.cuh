@@ -344,8 +344,8 @@ struct DecodeShape {
 // 32.2 -> 21.1; 384, 300: 17.4 -> 10.6; 4096, 300: 128 -> 105; 4096, 64: 59.5 -> 30.7; one K/V head
 // shared by 32 query heads, 64 keys: 5.4 -> 4.2.  Beyond 1024 keys the bandwidth evens the shapes out and
 // the rule of launch_decode is the better one (640 heads, 1500 keys: 93 by this rule, 89 by that one).
-inline DecodeShape decode_shape(int B, int H, int Sk, int D, bool shared_kv, int num_sms) {
-  if (Sk > 1024) return {shared_kv ? 4 : 1, 8, 0};
+inline DecodeShape decode_shape(int B, int H, int Sk, int D, bool shared_kv, int num_sms, bool any_length = false) {
+  if (Sk > 1024 && !any_length) return {shared_kv ? 4 : 1, 8, 0};
   const int rows = D <= 64 ? 32 : 16;  // rows of a warp's step
   DecodeShape best = {1, 8, 1};
   double best_cost = 0;
