@@ -82,9 +82,9 @@ SIGNATURES = {
                                                   _c.c_double, _c.c_double, _c.c_double, _c.c_double,
                                                   _PTR, _c.c_int, _PTR]),
     "fo_grad_norm": (_c.c_int, [_c.POINTER(_PTR), _I64P, _c.POINTER(_c.c_int), _c.c_int, _c.c_double,
-                                _PTR, _PTR, _PTR, _c.c_int, _PTR]),
+                                _PTR, _PTR, _PTR, _PTR, _c.c_int, _PTR]),
     "fo_grad_norm_workspace": (_c.c_int64, [_c.c_int]),
-    "fo_grad_norm_finish": (_c.c_int, [_PTR, _c.c_double, _PTR, _c.c_int, _PTR]),
+    "fo_grad_norm_finish": (_c.c_int, [_PTR, _c.c_double, _PTR, _PTR, _c.c_int, _PTR]),
     "fo_lion_clear_cache": (_c.c_int, []),
     "fo_launch_count": (_c.c_int64, []),
     "fo_debug_wait_timeout": (_c.c_int, [_c.c_int, _PTR, _c.c_int, _PTR]),

@@ -67,17 +67,17 @@ class GradList:
         self.dtypes = (ctypes.c_int * n)(*codes)
         self.doubles = _workspace_doubles(n)
 
-    def launch(self, max_norm: float, sumsq: Optional[Tensor] = None) -> Tensor:
-        """(norm, clipping factor) as two floats on the device; `sumsq`, if given, receives the sum of
-        squares as a double.  Workspace and result are allocated by the call, so that calls on
-        different streams or in different graphs share nothing."""
-        workspace = torch.empty(self.doubles, dtype=torch.float64, device=self.device)
-        result = torch.empty(2, dtype=torch.float32, device=self.device)
+    def launch(self, max_norm: float, sumsq: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        """The norm, a 0-d tensor, and a buffer whose first float is the clipping factor; `sumsq`, if
+        given, receives the sum of squares as a double.  All of it is allocated by the call, so that
+        calls on different streams or in different graphs share nothing."""
+        norm = torch.empty((), dtype=torch.float32, device=self.device)
+        buffer = torch.empty(self.doubles + 1, dtype=torch.float64, device=self.device)
+        coef = buffer.data_ptr()
         _lib.check(_lib.load().fo_grad_norm(
-            self.ptrs, self.numels, self.dtypes, self.n, max_norm, workspace.data_ptr(),
-            None if sumsq is None else sumsq.data_ptr(), result.data_ptr(), self.device_index,
-            _lib.current_stream_ptr(self.device_index)))
-        return result
+            self.ptrs, self.numels, self.dtypes, self.n, max_norm, coef + 8, None if sumsq is None else sumsq.data_ptr(),
+            norm.data_ptr(), coef, self.device_index, _lib.current_stream_ptr(self.device_index)))
+        return norm, buffer
 
 
 def grad_norm(grads: Iterable[Tensor]) -> Tensor:
@@ -95,12 +95,12 @@ def grad_norm(grads: Iterable[Tensor]) -> Tensor:
         return GradList(list(grads)).launch(float("inf"))[0]
 
 
-def finish_norm(sumsq: Tensor, max_norm: float) -> Tensor:
+def finish_norm(sumsq: Tensor, max_norm: float) -> Tuple[Tensor, Tensor]:
     """(norm, clipping factor) from a sum of squares (a double on the device)."""
-    result = torch.empty(2, dtype=torch.float32, device=sumsq.device)
-    _lib.check(_lib.load().fo_grad_norm_finish(sumsq.data_ptr(), max_norm, result.data_ptr(), sumsq.device.index,
-                                               _lib.current_stream_ptr(sumsq.device.index)))
-    return result
+    norm, coef = (torch.empty((), dtype=torch.float32, device=sumsq.device) for _ in range(2))
+    _lib.check(_lib.load().fo_grad_norm_finish(sumsq.data_ptr(), max_norm, norm.data_ptr(), coef.data_ptr(),
+                                               sumsq.device.index, _lib.current_stream_ptr(sumsq.device.index)))
+    return norm, coef
 
 
 def shard_sumsq(flat_g: Tensor, begin: int, end: int) -> Tensor:

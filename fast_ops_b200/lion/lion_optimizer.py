@@ -133,7 +133,9 @@ class Lion(Optimizer):
         self._momentum_dtype = momentum_dtype
         self._lists: Dict[int, tuple] = {}  # group index -> (address signature, prepared launches)
         self.max_grad_norm = max_grad_norm
-        self._norm_coef: Optional[Tensor] = None  # (norm, clipping factor) of the latest step
+        #: 0-d fp32 tensor: the norm of all gradients at the latest step, before clipping.  None before the
+        #: first step, without max_grad_norm, and after a step in which no parameter had a gradient
+        self.grad_norm: Optional[Tensor] = None
         self._grad_list: Optional[Tuple[list, Optional[GradList]]] = None
         self._pg = process_group
         self._zero = None
@@ -186,10 +188,9 @@ class Lion(Optimizer):
         lib = _lib.load()
         clip = None
         if self.max_grad_norm is not None:
-            self._norm_coef = self._launch_norm()
-            if self._norm_coef is None:
+            clip = self._clip_factor()
+            if clip is None:
                 return  # no parameter has a gradient
-            clip = self._norm_coef.data_ptr() + 4
         for gi, group in enumerate(self.param_groups):
             lr = float(group["lr"])
             weight_decay = float(group["weight_decay"])
@@ -202,7 +203,7 @@ class Lion(Optimizer):
                 if clip is None:
                     _lib.check(lib.fo_lion_multi_tensor_step(*args, *where))
                 else:
-                    _lib.check(lib.fo_lion_multi_tensor_step_clipped(*args, clip, *where))
+                    _lib.check(lib.fo_lion_multi_tensor_step_clipped(*args, clip.data_ptr(), *where))
 
     def _group_lists(self, gi: int, group) -> list:
         """The group's prepared launches.  A training loop presents the same tensors step after step:
@@ -215,23 +216,20 @@ class Lion(Optimizer):
             self._lists[gi] = cached
         return cached[1]
 
-    @property
-    def grad_norm(self) -> Optional[Tensor]:
-        """The norm of all gradients at the latest step, before clipping: a 0-d fp32 tensor.  None before
-        the first step, without `max_grad_norm`, and after a step in which no parameter had a gradient."""
-        return None if self._norm_coef is None else self._norm_coef[0]
-
-    def _launch_norm(self) -> Optional[Tensor]:
-        """Launches the norm over the gradients of all groups; returns (norm, clipping factor) on the
-        device, or None when no parameter has a gradient."""
+    def _clip_factor(self) -> Optional[Tensor]:
+        """Launches the norm over the gradients of all groups; returns a device buffer whose first float
+        is the clipping factor, or None when no parameter has a gradient."""
         max_norm = self._checked_max_norm()
         lists = [tl for gi, group in enumerate(self.param_groups) for tl in self._group_lists(gi, group)]
         if self._grad_list is None or len(self._grad_list[0]) != len(lists) or any(
                 a is not b for a, b in zip(self._grad_list[0], lists)):
             grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
             self._grad_list = (lists, GradList(grads) if grads else None)
-        grad_list = self._grad_list[1]
-        return None if grad_list is None else grad_list.launch(max_norm)
+        if self._grad_list[1] is None:
+            self.grad_norm = None
+            return None
+        self.grad_norm, buffer = self._grad_list[1].launch(max_norm)
+        return buffer
 
     def _checked_max_norm(self) -> float:
         max_norm = float(self.max_grad_norm)
@@ -356,9 +354,8 @@ class _Zero1State:
         sumsq = self.sumsq_fn(self.flat_g, self.begin, self.end)
         if self.world > 1:
             dist.all_reduce(sumsq, group=self.group)
-        result = self.finish_norm_fn(sumsq, max_norm)
-        self.opt._norm_coef = result
-        return result[1]
+        self.opt.grad_norm, coef = self.finish_norm_fn(sumsq, max_norm)
+        return coef
 
     @torch.no_grad()
     def step(self) -> None:

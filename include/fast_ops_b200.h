@@ -337,16 +337,16 @@ int fo_lion_flat_step_push_clipped(void* param, const void* grad, void* exp_avg_
  *   workspace  : device memory of fo_grad_norm_workspace(n_tensors) doubles, 8-byte aligned, not
  *                shared with a call that may run at the same time; contents on entry do not matter.
  *   sumsq      : device double that receives the sum of squares, or NULL.
- *   norm_coef  : two device floats that receive norm and coef, or NULL.
+ *   norm, coef : device floats that receive norm and coef, or NULL.
  */
 int fo_grad_norm(const void* const* grads, const int64_t* numels, const int* dtypes, int n_tensors,
-                 double max_norm, double* workspace, double* sumsq, float* norm_coef,
+                 double max_norm, double* workspace, double* sumsq, float* norm, float* coef,
                  int device, void* stream);
 int64_t fo_grad_norm_workspace(int n_tensors);
 
 /* Norm and coef, as fo_grad_norm writes them, from a sum of squares in device memory (one that has
  * been added up over the ranks of a sharded gradient). */
-int fo_grad_norm_finish(const double* sumsq, double max_norm, float* norm_coef, int device, void* stream);
+int fo_grad_norm_finish(const double* sumsq, double max_norm, float* norm, float* coef, int device, void* stream);
 
 /* Drops the cached tensor tables of fo_lion_multi_tensor_step (all devices). */
 int fo_lion_clear_cache(void);

@@ -33,7 +33,7 @@ def randoms(shapes, dtypes, seed=0, std=1e-2):
 @pytest.mark.parametrize("dtypes", [(FP,), (BF,), (HF,), (FP, BF, HF)])
 @pytest.mark.parametrize("shapes", [
     [(1,)], [(8192,)], [(8193,)], [(7,), (0,), (3, 5), (4097,), (12345,)], [(0,), (0,)], [(1 << 20,), (33,)],
-    [(257,)] * 95, [(31,)] * 96, [(1000 + i,) for i in range(97)], [(64,)] * 1024, [(5 + i % 7,) for i in range(2500)],
+    [(5000,)] * 32, [(5000,)] * 33, [(1 << 18,)], [((1 << 18) + 1,)], [(257,)] * 95, [(31,)] * 96, [(1000 + i,) for i in range(97)], [(64,)] * 1024, [(5 + i % 7,) for i in range(2500)],
 ])
 def test_norm_matches_64_bits(shapes, dtypes, cuda_device):
     gs = randoms(shapes, dtypes, seed=len(shapes))
@@ -276,7 +276,7 @@ def test_refused_entry_arguments(cuda_device):
     ptr, num, dt = (ctypes.c_void_p * 1)(t.data_ptr()), (ctypes.c_int64 * 1)(8), (ctypes.c_int * 1)(L.FO_F32)
     ws = torch.empty(lib.fo_grad_norm_workspace(1), dtype=torch.float64, device="cuda")
     out = torch.empty(2, device="cuda")
-    ok = (ptr, num, dt, 1, 1.0, ws.data_ptr(), None, out.data_ptr(), 0, None)
+    ok = (ptr, num, dt, 1, 1.0, ws.data_ptr(), None, out.data_ptr(), out.data_ptr() + 4, 0, None)
 
     def with_(i, v):
         a = list(ok)
@@ -284,9 +284,12 @@ def test_refused_entry_arguments(cuda_device):
         return lib.fo_grad_norm(*a)
 
     assert lib.fo_grad_norm(*ok) == 0
-    for i, v in ((3, -1), (4, -1.0), (4, math.nan), (5, None), (7, None), (0, (ctypes.c_void_p * 1)(None)),
+    for i, v in ((3, -1), (4, -1.0), (4, math.nan), (5, None), (0, (ctypes.c_void_p * 1)(None)),
                  (1, (ctypes.c_int64 * 1)(-1)), (2, (ctypes.c_int * 1)(7)), (0, (ctypes.c_void_p * 1)(t.data_ptr() + 2)),
                  (5, ws.data_ptr() + 4)):
         assert with_(i, v) == -1, i
+    assert lib.fo_grad_norm(ptr, num, dt, 1, 1.0, ws.data_ptr(), None, None, None, 0, None) == -1
+    for args in ((None, 1.0, out.data_ptr(), None), (ws.data_ptr(), 1.0, None, None), (ws.data_ptr(), -1.0, out.data_ptr(), None)):
+        assert lib.fo_grad_norm_finish(*args, 0, None) == -1
     torch.cuda.synchronize()
     assert out[0].item() == pytest.approx(math.sqrt(8), rel=1e-6) and out[1].item() == pytest.approx(1 / math.sqrt(8), rel=1e-6)
