@@ -50,8 +50,11 @@ struct Ws64sConfig {
   static constexpr int kOffRel = kOffBias + 2 * kStepN * 4;    // RelHead
   static constexpr int kOffRelVector = kOffRel + 32;            // the head's four copies of the bias vector
   static constexpr int kSmemBytes = kOffRelVector + 1024 /* alignment slack */;
-  // Longest copy of the vector that leaves room for two CTAs on an SM.
-  static constexpr int kMaxRelStride = (228 * 1024 / 2 - 1024 - kSmemBytes) / 16;
+  // Longest vector of which four copies, or two, leave room for two CTAs on an SM.
+  static constexpr int kRelRoom = 228 * 1024 / 2 - 1024 - kSmemBytes;
+  static constexpr int kMaxRelStride4 = kRelRoom / 16, kMaxRelStride2 = kRelRoom / 8;
+  // Copies that a launch keeps; 0: even two do not fit.
+  static int rel_copies(int stride) { return stride <= kMaxRelStride4 ? 4 : stride <= kMaxRelStride2 ? 2 : 0; }
   static constexpr uint32_t kTmemCols = 256;
   static constexpr uint32_t kColS = 0, kColO = 128;
 };
@@ -205,10 +208,10 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     float* const s_rel = reinterpret_cast<float*>(smem + Cfg::kOffRelVector);
     int rel_x = 0;  // where this row's bias of key 0 would be in its copy of the vector
     if constexpr (rel_bias) {
-      const int x = prm.rel.zero - row - q_off, s4 = x & 3;
-      rel_x = s4 * prm.rel.stride + (x - s4);
+      const int x = prm.rel.zero - row - q_off, shift = x & (prm.rel.smem_copies - 1);
+      rel_x = shift * prm.rel.stride + (x - shift);
       const float* const src = prm.rel.values + static_cast<int64_t>(h) * 4 * prm.rel.stride;
-      for (int i = r; i < prm.rel.stride; i += 128) cp_async16(s_rel + 4 * i, src + 4 * i);
+      for (int i = r; i < prm.rel.smem_copies * prm.rel.stride / 4; i += 128) cp_async16(s_rel + 4 * i, src + 4 * i);
     }
     // Copies step tn's values into their buffer, asynchronously, where they are not zero.
     auto fetch_vec = [&](int tn) {
@@ -254,7 +257,11 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           if constexpr (rel_bias) {
-            if (near) add_rel_bias<true>(sr[c], reinterpret_cast<const float4*>(s_rel + (rel_x + k0n + c * 32)));
+            if (near) {
+              const float* const p = s_rel + (rel_x + k0n + c * 32);
+              if (prm.rel.smem_copies == 4) add_rel_bias<true>(sr[c], reinterpret_cast<const float4*>(p));
+              else add_rel_bias_pairs(sr[c], reinterpret_cast<const float2*>(p));
+            }
             if (rel_vec && step_vec)
               add_rel_bias<true>(sr[c], reinterpret_cast<const float4*>(sb + (tn & 1) * kStepN + c * 32));
           }
@@ -504,8 +511,8 @@ template <int D, bool kBf16, int kMma = D, int kExt = 0>
 int launch_ws64s(const CUtensorMap& tq, const CUtensorMap& tk_half, const CUtensorMap& tv_half, const AttnParams& prm,
                  cudaStream_t stream) {
   auto kernel = attn_fwd_ws64s_kernel<D, kBf16, kMma, kExt>;
-  constexpr int most = Ws64sConfig<D>::kSmemBytes + (kExt != 0 ? 16 * Ws64sConfig<D>::kMaxRelStride : 0);
-  const int smem = Ws64sConfig<D>::kSmemBytes + (kExt != 0 ? 16 * prm.rel.stride : 0);
+  constexpr int most = Ws64sConfig<D>::kSmemBytes + (kExt != 0 ? Ws64sConfig<D>::kRelRoom : 0);
+  const int smem = Ws64sConfig<D>::kSmemBytes + (kExt != 0 ? 4 * prm.rel.smem_copies * prm.rel.stride : 0);
   if (smem > most) return fail(FO_ERR_UNSUPPORTED, "the bias vector does not fit this kernel");
   cudaError_t ea = ensure_dynamic_smem<attn_fwd_ws64s_kernel<D, kBf16, kMma, kExt>>(most, prm.device);
   if (ea != cudaSuccess)

@@ -11,7 +11,7 @@
 // part of such a tile can.  A thread reads neighbouring values from a place of its own, 16 bytes at a time:
 // the vector is there four times, copy s shifted by s values, so that one of them is aligned for it
 // (64 values by 16 loads instead of 64).  The copies are 8 banks apart, so that from shared memory eight
-// threads read 32 banks.
+// threads read 32 banks; a vector too long for four copies there is kept in two.
 //
 // A vector bias beside it (key padding, as a rule) is brought into the same form, one row for each
 // batch and head that has its own, with what lets the kernels pass over most of it: the end of the keys that
@@ -24,7 +24,7 @@
 namespace fo {
 
 constexpr int kRelMaxStarts = 256;  // buckets of one side: they travel in kernel arguments
-constexpr int kRelMargin = 192;
+constexpr int kRelMargin = 104;
 
 struct RelBuckets {
   int starts[kRelMaxStarts];
@@ -61,6 +61,7 @@ struct RelBias {
   float* acc;
   float2* tile_sums;
   int width, zero, stride;
+  int smem_copies;       // copies that the kernel with the vector in shared memory keeps (2 or 4)
   const float* vec;          // [rows][rel_vec_width], or null without a vector bias
   const int4* vec_extent;    // [rows]: (keys up to the last one not masked, first step with a bias, step after the last, 0)
   int vec_row_b, vec_row_h;  // row of (b, h): b * vec_row_b + h * vec_row_h
@@ -106,6 +107,16 @@ __device__ __forceinline__ void add_rel_bias(uint32_t (&s)[32], const float4* bi
     s[4 * i + 1] = __float_as_uint(lo.y);
     s[4 * i + 2] = __float_as_uint(hi.x);
     s[4 * i + 3] = __float_as_uint(hi.y);
+  }
+}
+
+// The same from an 8-byte aligned place in shared memory.
+__device__ __forceinline__ void add_rel_bias_pairs(uint32_t (&s)[32], const float2* bias) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 x = __fadd2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), bias[i]);
+    s[2 * i] = __float_as_uint(x.x);
+    s[2 * i + 1] = __float_as_uint(x.y);
   }
 }
 
