@@ -161,8 +161,9 @@ class _Call:
     def backward(self, dO: Tensor, Q: Tensor, K: Tensor, V: Tensor, O: Tensor, LSE: Tensor, workspace: Tensor,
                  bias: Optional[Tensor], table_grad: Optional[torch.dtype]):
         """(dQ, dK, dV, the table's gradient or None)."""
-        if dO.stride(3) != 1:
-            dO = dO.contiguous()
+        sb, sh, ss, sd = dO.stride()
+        if sd != 1 or sb % 8 or sh % 8 or ss % 8 or not (sb and sh and ss) or dO.data_ptr() % 16:
+            dO = dO.contiguous()  # broadcast or cut from a larger tensor
         if K.stride(1) == 0 or V.stride(1) == 0:
             # one K/V head for all query heads: one dK, dV per query head needs storage of its own
             # (autograd sums them through the expand)

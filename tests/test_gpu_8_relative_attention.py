@@ -472,3 +472,90 @@ def test_both_forward_kernels(impl, D, dtype, causal, cuda_device):
             check_train(Q, K, V, table, dO, max_distance=128, bidirectional=not causal, causal=causal, bias=bias)
     finally:
         L.attn_configure(impl="auto")
+
+
+def test_output_gradients_that_are_broadcast_or_cut(cuda_device):
+    Q, K, V, table, dO = make(2, 2, 100, 100, 64, BF, 32)
+    leaves = [t.clone().requires_grad_() for t in (Q, K, V, table)]
+    O = relative_attention(*leaves)
+    for g in (torch.ones((), device="cuda", dtype=BF).expand_as(O), dO[:1].expand_as(O), dO[:, :, :1].expand_as(O),
+              torch.randn(2, 2, 100, 65, device="cuda", dtype=BF)[..., 1:]):
+        got = torch.autograd.grad(O, leaves, g, retain_graph=True)
+        want = torch.autograd.grad(O, leaves, g.contiguous(), retain_graph=True)
+        for i in (1, 2, 3):
+            assert torch.equal(got[i], want[i])
+        assert torch.allclose(got[0].float(), want[0].float(), rtol=2.0**-7, atol=1e-6)  # dQ is summed by atomic adds
+
+
+def test_packed_projections(cuda_device):
+    """Q, K and V as views of one (B, S, 3, H, D) tensor, whose gradient collects theirs."""
+    B, H, S, D = 2, 3, 130, 64
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    qkv = torch.empty(B, S, 3, H, D, dtype=BF, device="cuda").normal_(generator=gen).requires_grad_()
+    table = torch.empty(32, H, dtype=BF, device="cuda").normal_(generator=gen).requires_grad_()
+    dO = torch.empty(B, H, S, D, dtype=BF, device="cuda").normal_(generator=gen)
+    q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
+    O = relative_attention(q, k, v, table)
+    g, dT = torch.autograd.grad(O, (qkv, table), dO)
+    want, tol = formula(*(t.detach().contiguous() for t in (q, k, v)), table, dO, max_distance=128, bidirectional=True)
+    want, tol = ({n: x.detach() for n, x in d.items()} for d in (want, tol))
+    close("O", O.detach(), want["O"], tol["O"])
+    for i, name in enumerate(("dQ", "dK", "dV")):
+        close(name, g[:, :, i].transpose(1, 2), want[name], tol[name])
+    close("dT", dT, want["dT"], tol["dT"])
+
+
+def test_two_streams_at_once(cuda_device):
+    """Calls of different problems that run side by side share nothing."""
+    problems = [make(2, 4, 500, 500, 64, BF, 32, seed=i) for i in range(2)]
+    want = [train(*p) for p in problems]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in problems]
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(train(*problems[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            for x in (0, 1, 3, 4, 5):
+                assert torch.equal(g[x], want[i][x])
+
+
+def test_a_step_of_attention_clipping_and_lion(cuda_device):
+    """The operators together, as a training loop uses them: attention with a learned bias, its table's gradient
+    among those whose norm clips the step.  Each part against its formula from what the part before it gave."""
+    from fast_ops_b200.lion import Lion
+
+    B, H, S, D = 2, 4, 200, 64
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(B, S, H * D, dtype=BF, device="cuda").normal_(generator=gen)
+    weights = [torch.nn.Parameter(torch.empty(H * D, H * D, dtype=BF, device="cuda").normal_(0, (H * D) ** -0.5, generator=gen))
+               for _ in range(3)]
+    table = torch.nn.Parameter(torch.empty(32, H, dtype=BF, device="cuda").normal_(generator=gen))
+    params = weights + [table]
+    opt = Lion(params, lr=1e-3, weight_decay=0.1, max_grad_norm=0.5)
+    for step in range(3):
+        q, k, v = ((x @ w.T).view(B, S, H, D).transpose(1, 2) for w in weights)
+        O = relative_attention(q, k, v, table, bias=padding(B, S, (150, 200)), causal=False)
+        dO = torch.empty_like(O).normal_(generator=gen)
+        before = [p.detach().clone() for p in params]
+        momenta = [opt.state[p]["exp_avg"].clone() if step else torch.zeros_like(p) for p in params]
+        opt.zero_grad(set_to_none=True)
+        O.backward(dO)
+        want, tol = formula(*(t.detach().contiguous() for t in (q, k, v)), table.detach(), dO, max_distance=128,
+                            bidirectional=True, bias=padding(B, S, (150, 200)))
+        close("O", O.detach(), want["O"], tol["O"])
+        close("dT", table.grad, want["dT"], tol["dT"])
+        opt.step()
+        norm = math.sqrt(sum(p.grad.double().square().sum().item() for p in params))
+        assert abs(opt.grad_norm.item() - norm) <= 4.5 * 2.0**-24 * norm and norm > 0.5
+        coef = torch.full((), 0.5, device="cuda") / (opt.grad_norm + 1e-6)
+        for p, p0, m0 in zip(params, before, momenta):
+            rp, rm = torch.nn.Parameter(p0), m0
+            rp.grad = (p.grad.float() * coef).to(BF)
+            ref = Lion([rp], lr=1e-3, weight_decay=0.1)
+            ref.state[rp]["exp_avg"] = rm
+            ref.step()
+            assert torch.equal(p, rp) and torch.equal(opt.state[p]["exp_avg"], rm)
