@@ -55,12 +55,17 @@ attn_bwd_prepare_kernel(const uint16_t* __restrict__ o, const uint16_t* __restri
 }
 
 // dQ = round(dq_accum) in the input type.  One thread per 8 elements.
-template <bool kBf16>
+// kOverlap: launched so that it may run beside the kernel before it on the stream, on which it does not depend; its
+// blocks end behind that kernel's, so that what follows on the stream waits for both.
+template <bool kBf16, bool kOverlap = false>
 __global__ void __launch_bounds__(256)
 attn_bwd_finish_dq_kernel(const float* __restrict__ dq_accum, uint16_t* __restrict__ dq, int H, int Sq, int D,
                           int64_t q_sb, int64_t q_sh, int64_t q_ss, int64_t groups) {
   const int64_t g = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (g >= groups) return;
+  if (g >= groups) {
+    if constexpr (kOverlap) fo::grid_wait_previous();
+    return;
+  }
   const int per_row = D / 8;
   const int64_t r = g / per_row;
   const int d0 = static_cast<int>(g - r * per_row) * 8;
@@ -75,6 +80,7 @@ attn_bwd_finish_dq_kernel(const float* __restrict__ dq_accum, uint16_t* __restri
   v.z = fo::pack2<kBf16>(a1.x, a1.y);
   v.w = fo::pack2<kBf16>(a1.z, a1.w);
   *reinterpret_cast<uint4*>(dq + b * q_sb + h * q_sh + row * q_ss + d0) = v;
+  if constexpr (kOverlap) fo::grid_wait_previous();
 }
 
 int check_out_strides(const int64_t s[3], const char* name) {
@@ -202,7 +208,12 @@ int fo::attn_bwd_impl(const void* q, const void* k, const void* v, const void* o
     const int64_t groups = rows * (D / 8);
     const unsigned blocks = static_cast<unsigned>((groups + 255) / 256);
     auto* dqp = static_cast<uint16_t*>(dq);
-    if (bf16)
+    if (rel && rel->dtable != nullptr) {
+      if (int rc2 = fo::launch_table_grad(*rel, B, H, Sq, Sk, D, causal, softmax_scale, prm.ex.dropout != 0, s)) return rc2;
+      auto kernel = bf16 ? attn_bwd_finish_dq_kernel<true, true> : attn_bwd_finish_dq_kernel<false, true>;
+      FO_CUDA_CHECK(fo::launch_overlapping(kernel, dim3(blocks), dim3(256), 0, s, static_cast<const float*>(dq_accum), dqp, H, Sq,
+                                           D, dq_strides[0], dq_strides[1], dq_strides[2], groups));
+    } else if (bf16)
       attn_bwd_finish_dq_kernel<true><<<blocks, 256, 0, s>>>(dq_accum, dqp, H, Sq, D, dq_strides[0], dq_strides[1],
                                                              dq_strides[2], groups);
     else

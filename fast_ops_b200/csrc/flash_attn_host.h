@@ -19,6 +19,8 @@ struct RelArgs {
   int64_t stride_bucket, stride_head;  // elements
   int table_f32;                       // 1: fp32, 0: the 16-bit type of q
   RelBias bias;                        // what the tile kernels read
+  void* dtable;                        // backward: the table's gradient, of table_dtype, or null
+  int table_dtype;
   int64_t bias_rows;                   // rows of the expanded vector bias, of bias_heads heads each
   int bias_heads;
 };
@@ -47,6 +49,10 @@ int launch_fwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
 int launch_bwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                    const CUtensorMap& tdq, const AttnBwdParams& prm, bool bf16, cudaStream_t stream);
 int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, float softmax_scale, bool bf16,
+                      cudaStream_t stream);
+
+// The table's gradient from the partial sums of launch_bwd_rel's kernel.
+int launch_table_grad(const RelArgs& rel, int B, int H, int Sq, int Sk, int D, int causal, float softmax_scale, bool dropout,
                       cudaStream_t stream);
 
 struct DecodeParams;

@@ -43,6 +43,7 @@ struct ExpandParams {
 template <bool kBf16>
 __global__ void __launch_bounds__(256)
 rel_expand_kernel(const __grid_constant__ ExpandParams prm) {
+  fo::grid_allow_next();
   const int per_head = (prm.width + 255) / 256;
   if (static_cast<int>(blockIdx.x) < prm.value_blocks) {
     const int h = blockIdx.x / per_head;
@@ -117,6 +118,7 @@ __global__ void __cluster_dims__(kGradCtas, 1, 1) __launch_bounds__(kGradWarps *
 rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, int n_q_tiles, int n_k_tiles, int warps,
                       int causal, float inv_scale) {
   namespace cg = cooperative_groups;
+  fo::grid_allow_next();  // the rounding of dQ, which does not depend on this
   cg::cluster_group cluster = cg::this_cluster();
   __shared__ double far[kGradWarps][2];
   __shared__ double cta_far[2];
@@ -376,6 +378,23 @@ int launch_bwd_rel(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorM
 #undef FO_REL_FORM
 }
 
+int launch_table_grad(const RelArgs& rel, int B, int H, int Sq, int Sk, int D, int causal, float softmax_scale, bool dropout,
+                      cudaStream_t stream) {
+  const int q_tiles = (Sq + kBlockM - 1) / kBlockM, k_tiles = (Sk + kBlockN - 1) / kBlockN;
+  const int warps = bwd_warps(D, dropout);
+  const float inv = 1.f / softmax_scale;
+#define FO_TABLE_GRAD(T)                                                       \
+  rel_table_grad_kernel<<<dim3(kGradCtas, H), kGradWarps * 32, 0, stream>>>(   \
+      rel.bias, static_cast<T*>(rel.dtable), B, H, q_tiles, k_tiles, warps, causal ? 1 : 0, inv)
+  if (rel.table_dtype == FO_F32) FO_TABLE_GRAD(float);
+  else if (rel.table_dtype == FO_BF16) FO_TABLE_GRAD(__nv_bfloat16);
+  else FO_TABLE_GRAD(__half);
+#undef FO_TABLE_GRAD
+  g_launch_count.fetch_add(1, std::memory_order_relaxed);
+  FO_CUDA_CHECK(cudaGetLastError());
+  return FO_OK;
+}
+
 int launch_decode_rel(const DecodeParams& prm, const RelArgs& args, const AttnExtras& ex, int B, int H, int Sk, int D,
                       bool shared_kv, bool bf16, int num_sms, int device, cudaStream_t stream) {
   DecodeRel rel;
@@ -480,7 +499,12 @@ extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, cons
   fo::AttnExtras ex;
   if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset)) return rc;
   if (int rc = set_expanded(&rel, const_cast<void*>(workspace), ex, B, H, Sk, true)) return rc;
+  rel.dtable = dtable;
+  rel.table_dtype = table_dtype;
   if (dtable != nullptr) {
+    FO_REQUIRE(4LL * B * ((Sq + fo::kBlockM - 1) / fo::kBlockM) < (1LL << 31) &&
+                   1LL * B * ((Sk + fo::kBlockN - 1) / fo::kBlockN) * 16 < (1LL << 31),
+               "too many tiles for the table's gradient");
     rel.bias.tile_sums = reinterpret_cast<float2*>(partials);
     rel.bias.acc = partials + tile_sum_floats(B, H, Sq, Sk, D, ex.dropout != 0);
   }
@@ -488,21 +512,5 @@ extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, cons
                                  v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides, dtype, causal,
                                  softmax_scale, &ex, &rel, device, stream))
     return rc;
-  if (dtable == nullptr) return FO_OK;
-  fo::DeviceGuard guard(device);
-  FO_REQUIRE(guard.ok, "cannot make device %d current", device);
-  const int q_tiles = (Sq + fo::kBlockM - 1) / fo::kBlockM, k_tiles = (Sk + fo::kBlockN - 1) / fo::kBlockN;
-  const int warps = bwd_warps(D, ex.dropout != 0);
-  FO_REQUIRE(4LL * B * q_tiles < (1LL << 31) && 1LL * B * k_tiles * warps < (1LL << 31), "too many tiles for the table's gradient");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const float inv = 1.f / softmax_scale;
-#define FO_TABLE_GRAD(T)                                                                                             \
-  rel_table_grad_kernel<<<dim3(kGradCtas, H), kGradWarps * 32, 0, s>>>(rel.bias, static_cast<T*>(dtable), B, H, q_tiles, k_tiles, warps, causal ? 1 : 0, inv)
-  if (table_dtype == FO_F32) FO_TABLE_GRAD(float);
-  else if (table_dtype == FO_BF16) FO_TABLE_GRAD(__nv_bfloat16);
-  else FO_TABLE_GRAD(__half);
-#undef FO_TABLE_GRAD
-  fo::g_launch_count.fetch_add(1, std::memory_order_relaxed);
-  FO_CUDA_CHECK(cudaGetLastError());
   return FO_OK;
 }

@@ -117,6 +117,9 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
   const int q0 = q_tile * kBlockM;
   constexpr bool rel_bias = (kExt & kFwdRelBias) != 0, rel_vec = rel_bias && (kExt & kFwdVecBias) != 0;
   const int q_off = rel_bias ? prm.rel.offset : 0;  // query row i stands at key position i + q_off
+  // A relative bias: the launch overlaps the kernel that expands the bias, and waits for it where it first reads
+  // what that writes.
+  if constexpr (rel_vec) grid_wait_previous();
   const int keys = rel_bias ? rel_keys(prm.rel, b, h, prm.Sk) : prm.Sk;
   const int vis = prm.causal ? min(keys, q0 + kBlockM + q_off) : keys;  // keys this tile sees
   const int T = (vis + kStepN - 1) / kStepN;                       // 64-key steps, >= 1
@@ -179,6 +182,7 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
     tmem_relinquish_alloc_permit();
   }
   if (rel_bias && tid == 0) {
+    grid_wait_previous();
     RelHead head = {rel_value(prm.rel, h, -prm.rel.zero) * prm.scale_log2, rel_value(prm.rel, h, prm.rel.width) * prm.scale_log2, 0, 0, 0};
     if constexpr (rel_vec) {
       head.vec_row = static_cast<int>(rel_vec_row(prm.rel, b, h));
@@ -211,6 +215,7 @@ attn_fwd_ws64s_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       const int x = prm.rel.zero - row - q_off, shift = x & (prm.rel.smem_copies - 1);
       rel_x = shift * prm.rel.stride + (x - shift);
       const float* const src = prm.rel.values + static_cast<int64_t>(h) * 4 * prm.rel.stride;
+      grid_wait_previous();
       for (int i = r; i < prm.rel.smem_copies * prm.rel.stride / 4; i += 128) cp_async16(s_rel + 4 * i, src + 4 * i);
     }
     // Copies step tn's values into their buffer, asynchronously, where they are not zero.
@@ -519,9 +524,14 @@ int launch_ws64s(const CUtensorMap& tq, const CUtensorMap& tk_half, const CUtens
     return fail(FO_ERR_CUDA, "cudaFuncSetAttribute(shared memory %d) failed: %s", smem, cudaGetErrorString(ea));
   const int64_t blocks = static_cast<int64_t>(prm.num_q_tiles) * prm.B * prm.H;
   if (blocks > 0x7fffffffLL) return fail(FO_ERR_INVALID_ARGUMENT, "too many query tiles for one launch");
-  kernel<<<static_cast<unsigned>(blocks), 192, smem, stream>>>(tq, tk_half, tv_half, prm);
+  cudaError_t e;
+  if constexpr (kExt != 0) {
+    e = launch_overlapping(kernel, dim3(static_cast<unsigned>(blocks)), dim3(192), smem, stream, tq, tk_half, tv_half, prm);
+  } else {
+    kernel<<<static_cast<unsigned>(blocks), 192, smem, stream>>>(tq, tk_half, tv_half, prm);
+    e = cudaGetLastError();
+  }
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
-  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(FO_ERR_CUDA, "attention launch failed: %s", cudaGetErrorString(e));
   return FO_OK;
 }

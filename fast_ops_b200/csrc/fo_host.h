@@ -46,6 +46,23 @@ inline cudaError_t ensure_dynamic_smem(int bytes, int device) {
   return e;
 }
 
+// Launches a kernel that may overlap the one before it on the stream (grid_wait_previous in fo_ptx.cuh).
+template <class... Params, class... Args>
+inline cudaError_t launch_overlapping(void (*kernel)(Params...), dim3 grid, dim3 block, int smem, cudaStream_t stream,
+                                      const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // RAII: make `device` current for the scope, restore the previous one afterwards.  The device is set
 // even when it already is the thread's device: a thread that has made no runtime call yet (an
 // autograd worker) has no context bound, and the driver call that encodes tensor maps needs one.

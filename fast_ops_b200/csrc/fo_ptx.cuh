@@ -163,6 +163,12 @@ template <int kRegs> __device__ __forceinline__ void reg_dealloc() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
+// Programmatic launches: a kernel launched so may start when every block of the kernel before it has called
+// grid_allow_next (or ended); what that kernel writes is there behind grid_wait_previous, which also returns at
+// once in a kernel launched in the ordinary way.
+__device__ __forceinline__ void grid_allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // 16 bytes from global to shared memory by the threads' own asynchronous copy, and the wait for all of a thread's.
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
