@@ -93,7 +93,7 @@ constexpr int kBwdVecBias = 1, kBwdDropout = 2, kBwdMatBias = 4, kBwdRelBias = 8
 
 template <int D, int kExt>
 struct BwdConfig {
-  // head_dim 64 with dropout or a matrix bias: sixteen compute warps (four threads per key row, 32
+  // head_dim 64 with dropout, a matrix bias or a relative one: sixteen compute warps (four threads per key row, 32
   // query columns each) instead of eight.  Hashing and fetching bias values are long chains per
   // thread, and eight warps do not cover their latency.  us, whole backward, B2 H16 S2048 / B8 H12 S1024
   // causal / B32 H12 S128, before this form and with it: dropout 300 and 234 / 181 and 138 / 43 and 36;
@@ -101,8 +101,10 @@ struct BwdConfig {
   // 32 at a time: 2048 and 264 / 582 and 132 / 75 and 34, with dropout 2160 and 392 / 636 and 190 / 81 and
   // 41.)  The compiler spills 24 to 84 bytes in all four.  Without dropout or a matrix bias eight warps are
   // the faster form (B8 H12 S1024 D64 causal 81 against 84 us), and at head_dim 128 the registers do not
-  // reach.
-  static constexpr bool kWide = D == 64 && (kExt & (kBwdDropout | kBwdMatBias)) != 0;
+  // reach.  A relative bias (two-sided, 32 buckets to distance 128), whole backward with the table's gradient,
+  // eight and sixteen warps: B8 H12 S1024 174 and 162, B16 H12 S512 120 and 116; without that gradient 133 and
+  // 134, 91 and 93.
+  static constexpr bool kWide = D == 64 && (kExt & (kBwdDropout | kBwdMatBias | kBwdRelBias)) != 0;
   static constexpr int kComputeWarps = kWide ? 16 : 8;
   static constexpr int kThreads = kComputeWarps * 32 + 256;
   static constexpr int kCols = 128 * 4 / kComputeWarps;  // query columns of one compute thread
