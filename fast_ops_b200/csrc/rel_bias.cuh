@@ -6,9 +6,8 @@
 //
 // The tile kernels read the bias of a head as a vector over the relative position d = j - i - offset, at
 // x = d + zero, divided by the softmax scale: it is added to Q K^T, and the scale in the exponent applies to both.
-// It is constant from -far_left down and from far_right up, so that only the
-// tiles near the diagonal read it at all; its ends reach kRelMargin further, which is more than a warp's
-// part of such a tile can.  A thread reads neighbouring values from a place of its own, 16 bytes at a time:
+// It is constant from -far_left down and from far_right up, so that only the tiles near the diagonal read it at
+// all; its ends reach kRelMargin further, which is more than a warp's part of such a tile can.  A thread reads neighbouring values from a place of its own, 16 bytes at a time:
 // the vector is there four times, copy s shifted by s values, so that one of them is aligned for it
 // (64 values by 16 loads instead of 64).  The copies are 8 banks apart, so that from shared memory eight
 // threads read 32 banks; a vector too long for four copies there is kept in two.
@@ -61,7 +60,7 @@ struct RelBias {
   float* acc;
   float2* tile_sums;
   int width, zero, stride;
-  int smem_copies;       // copies that the kernel with the vector in shared memory keeps (2 or 4)
+  int smem_copies;           // copies that the kernel with the vector in shared memory keeps (2 or 4)
   const float* vec;          // [rows][rel_vec_width], or null without a vector bias
   const int4* vec_extent;    // [rows]: (keys up to the last one not masked, first step with a bias, step after the last, 0)
   int vec_row_b, vec_row_h;  // row of (b, h): b * vec_row_b + h * vec_row_h
@@ -77,10 +76,12 @@ __device__ __forceinline__ RelSide rel_side(const RelBias& rel, int first, int l
   return last <= -rel.far_left ? kRelLeft : first >= rel.far_right ? kRelRight : kRelNear;
 }
 
-// Bias (divided by the softmax scale) of relative position d for head h, whatever d is.
+// Bias (divided by the softmax scale) of relative position d for head h, whatever d is.  (This and the row's extent
+// below are not read as constant data, __ldg: a kernel whose launch overlaps the expansion starts before they are
+// written.)
 __device__ __forceinline__ float rel_value(const RelBias& rel, int h, int d) {
   const int x = min(max(d, -rel.zero), rel.width - 1 - rel.zero) + rel.zero;
-  return __ldg(rel.values + static_cast<int64_t>(h) * 4 * rel.stride + x);
+  return __ldcg(rel.values + static_cast<int64_t>(h) * 4 * rel.stride + x);
 }
 
 // Row of the vector bias, and the keys that a head computes: `keys`, or those up to the last one not masked, but
@@ -89,7 +90,7 @@ __device__ __forceinline__ int64_t rel_vec_row(const RelBias& rel, int b, int h)
   return static_cast<int64_t>(b) * rel.vec_row_b + static_cast<int64_t>(h) * rel.vec_row_h;
 }
 __device__ __forceinline__ int rel_keys(const RelBias& rel, int b, int h, int keys) {
-  return rel.vec == nullptr ? keys : min(keys, max(__ldg(&rel.vec_extent[rel_vec_row(rel, b, h)].x), 1));
+  return rel.vec == nullptr ? keys : min(keys, max(__ldcg(&rel.vec_extent[rel_vec_row(rel, b, h)].x), 1));
 }
 
 // Keys of a row of `vec`: whole key tiles.
