@@ -300,32 +300,32 @@ attn_decode_kernel(const DecodeParams prm, const __grid_constant__ Rel rel) {
   cluster.sync();  // no CTA leaves while its shared memory is being read
 }
 
-// CTAs of this kernel that can be resident together in clusters of 16 (asked once per device; the
-// largest cluster must find all its SMs inside one GPC, so the chip holds fewer of them).
+// CTAs of this kernel that can be resident together in clusters of `size` (asked once per device and size; a
+// cluster must find all its SMs inside one GPC, so the chip holds fewer of the larger ones).
 template <auto kKernel, int kThreads>
-inline int resident_ctas_in_clusters_of_16(int device) {
-  static std::atomic<int> known[64];  // CTAs + 1, 0 = not asked yet
-  if (device < 0 || device >= 64) return 0;
-  int n = known[device].load(std::memory_order_acquire);
+inline int resident_ctas_in_clusters(int device, int size) {
+  static std::atomic<int> known[64][17];  // CTAs + 1, 0 = not asked yet
+  if (device < 0 || device >= 64 || size < 1 || size > 16) return 0;
+  int n = known[device][size].load(std::memory_order_acquire);
   if (n == 0) {
     int clusters = 0;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(16);
+    cfg.gridDim = dim3(size);
     cfg.blockDim = dim3(kThreads);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 16;
+    attr[0].val.clusterDim.x = size;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+    if ((size > 8 && cudaFuncSetAttribute(kKernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) ||
         cudaOccupancyMaxActiveClusters(&clusters, kKernel, &cfg) != cudaSuccess) {
-      cudaGetLastError();  // not an error of the call: clusters of 16 are not used
+      cudaGetLastError();  // not an error of the call: clusters of this size are not used
       clusters = 0;
     }
-    n = clusters * 16 + 1;
-    known[device].store(n, std::memory_order_release);
+    n = clusters * size + 1;
+    known[device][size].store(n, std::memory_order_release);
   }
   return n - 1;
 }
@@ -344,8 +344,8 @@ struct DecodeShape {
 // 32.2 -> 21.1; 384, 300: 17.4 -> 10.6; 4096, 300: 128 -> 105; 4096, 64: 59.5 -> 30.7; one K/V head
 // shared by 32 query heads, 64 keys: 5.4 -> 4.2.  Beyond 1024 keys the bandwidth evens the shapes out and
 // the rule of launch_decode is the better one (640 heads, 1500 keys: 93 by this rule, 89 by that one).
-inline DecodeShape decode_shape(int B, int H, int Sk, int D, bool shared_kv, int num_sms, bool any_length = false) {
-  if (Sk > 1024 && !any_length) return {shared_kv ? 4 : 1, 8, 0};
+inline DecodeShape decode_shape(int B, int H, int Sk, int D, bool shared_kv, int num_sms) {
+  if (Sk > 1024) return {shared_kv ? 4 : 1, 8, 0};
   const int rows = D <= 64 ? 32 : 16;  // rows of a warp's step
   DecodeShape best = {1, 8, 1};
   double best_cost = 0;
@@ -378,7 +378,7 @@ int launch_decode(const DecodeParams& base, const Rel& rel, int B, int split, in
     const int resident = num_sms * kDecodePerSm<kHeads, kWarps>;
     double best = 0;
     for (int s = 1; s <= 16 && (s == 1 || base.Sk / s >= 128); s *= 2) {
-      const int slots = s == 16 ? resident_ctas_in_clusters_of_16<kernel, kWarps * 32>(device) : resident;
+      const int slots = s == 16 ? resident_ctas_in_clusters<kernel, kWarps * 32>(device, 16) : resident;
       if (slots < s) break;
       const double cost = static_cast<double>((groups * s + slots - 1) / slots) / s;
       if (s == 1 || cost < 0.85 * best) {
@@ -403,6 +403,54 @@ int launch_decode(const DecodeParams& base, const Rel& rel, int B, int split, in
   FO_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, prm, rel));
   g_launch_count.fetch_add(1, std::memory_order_relaxed);
   return FO_OK;
+}
+
+// The same cost over all lengths, with every cluster size and the CTAs that are really resident in clusters of it:
+// the rule of the kernels with a bias.  us against the rules above (the cost of the choice is the least, or within
+// 5 % of it): B16 H12 Sk2048 D64 24.7 and 20.9; B5 H16 Sk1500 D128 22.4 and 14.3; B7 H12 Sk10000 D128 79 and 68; B8
+// H12 Sk3000 D64 22.7 and 16.5; B32 H32 Sk2000 D64 91 and 84; one K/V head for 16, B12 Sk4500 D64 36 and 21;
+// within 2 % where few heads or short keys leave no choice.
+template <int D, bool kBf16, class Rel>
+int launch_decode_best(const DecodeParams& prm, const Rel& rel, int B, int Sk, bool shared_kv, int num_sms, int device,
+                       cudaStream_t stream) {
+  const int rows = D <= 64 ? 32 : 16;  // rows of a warp's step
+  int best[3] = {1, 8, 1};
+  double best_cost = 0;
+  auto consider = [&](auto heads_c, auto warps_c) {
+    constexpr int kHeads = heads_c.value, kWarps = warps_c.value;
+    const int64_t groups = static_cast<int64_t>((prm.H + kHeads - 1) / kHeads) * B;
+    for (int split = 1; split <= 16; split = split == 8 ? 16 : split + 1) {
+      if (split > 1 && Sk / split < (split > 8 ? 128 : 64)) break;
+      const int steps = (Sk + split * rows * kWarps - 1) / (split * rows * kWarps);
+      const double round = steps * (kHeads == 1 ? 1.0 : 1.3) + 4;
+      const int64_t ctas = groups * split;
+      const int64_t most = num_sms * kDecodePerSm<kHeads, kWarps>;  // what could be resident at best
+      if (best_cost != 0 && (ctas + most - 1) / most * round >= 0.95 * best_cost) continue;
+      const int64_t slots = split == 1 ? most : resident_ctas_in_clusters<attn_decode_kernel<D, kBf16, kHeads, kWarps, Rel>, kWarps * 32>(device, split);
+      if (slots < split) continue;
+      const double cost = static_cast<double>((ctas + slots - 1) / slots) * round;
+      if (best_cost == 0 || cost < 0.95 * best_cost) {
+        best_cost = cost;
+        best[0] = kHeads;
+        best[1] = kWarps;
+        best[2] = split;
+      }
+    }
+  };
+  using std::integral_constant;
+  consider(integral_constant<int, 1>{}, integral_constant<int, 8>{});
+  consider(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+  consider(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+  if (shared_kv) {
+    consider(integral_constant<int, 4>{}, integral_constant<int, 8>{});
+    consider(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    consider(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+  }
+#define FO_DECODE(HEADS, WARPS)                  \
+  if (best[0] == HEADS && best[1] == WARPS) return launch_decode<D, kBf16, HEADS, WARPS>(prm, rel, B, best[2], num_sms, device, stream);
+  FO_DECODE(1, 8) FO_DECODE(1, 4) FO_DECODE(1, 2) FO_DECODE(4, 8) FO_DECODE(4, 4) FO_DECODE(4, 2)
+#undef FO_DECODE
+  return fail(FO_ERR_UNSUPPORTED, "no decoding kernel of this shape");
 }
 
 }  // namespace fo

@@ -408,23 +408,10 @@ int launch_decode_rel(const DecodeParams& prm, const RelArgs& args, const AttnEx
   rel.bias_stride_b = ex.bias_stride_b;
   rel.bias_stride_h = ex.bias_stride_h;
   rel.bias_f32 = ex.bias_f32;
-  // The same rule for all lengths (us, B16 H12 Sk2048 D64: 21.3 with one CTA of eight warps per head, 24.7 with
-  // four as launch_decode splits long keys; B32 H32 Sk2000 D64 84 and 91; over nine shapes never more than 2 %
-  // behind), but few heads over long keys leave the split to launch_decode, which knows clusters of 16.
-  DecodeShape shape = decode_shape(B, H, Sk, D, shared_kv, num_sms, true);
-  if (shape.split == 8 && Sk >= 2048) shape = {shared_kv ? 4 : 1, 8, 0};
-#define FO_DECODE(DK, HEADS, WARPS)                                                                                     \
-  if ((DK == 64) == (D <= 64) && shape.heads == HEADS && shape.warps == WARPS)                                          \
-    return bf16 ? launch_decode<DK, true, HEADS, WARPS>(prm, rel, B, shape.split, num_sms, device, stream)              \
-                : launch_decode<DK, false, HEADS, WARPS>(prm, rel, B, shape.split, num_sms, device, stream);
-#define FO_DECODE_WARPS(DK, HEADS) FO_DECODE(DK, HEADS, 8) FO_DECODE(DK, HEADS, 4) FO_DECODE(DK, HEADS, 2)
-  FO_DECODE_WARPS(64, 1)
-  FO_DECODE_WARPS(64, 4)
-  FO_DECODE_WARPS(128, 1)
-  FO_DECODE_WARPS(128, 4)
-#undef FO_DECODE_WARPS
-#undef FO_DECODE
-  return fail(FO_ERR_UNSUPPORTED, "no decoding kernel of this shape");
+  if (D <= 64) return bf16 ? launch_decode_best<64, true>(prm, rel, B, Sk, shared_kv, num_sms, device, stream)
+                           : launch_decode_best<64, false>(prm, rel, B, Sk, shared_kv, num_sms, device, stream);
+  return bf16 ? launch_decode_best<128, true>(prm, rel, B, Sk, shared_kv, num_sms, device, stream)
+              : launch_decode_best<128, false>(prm, rel, B, Sk, shared_kv, num_sms, device, stream);
 }
 
 }  // namespace fo
