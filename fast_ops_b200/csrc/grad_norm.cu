@@ -192,10 +192,11 @@ grad_sumsq_kernel(const __grid_constant__ TensorList<kMax> list, double* __restr
   if (threadIdx.x == 0) partials[blockIdx.x] = sum;
 }
 
-// A short list in one launch: a cluster of blocks, the first of which adds up what the others have.  (8192 bf16
-// elements: 3.2 us instead of 3.5 + 2.8, and one launch less for the host.)
+// A short list in one launch: a cluster of blocks, the first of which adds up what the others have.  Back to back in a
+// graph, bf16, this and the two launches: 8192 elements 2.6 and 2.8 us, 65536 2.8 and 3.2, 131072 3.6 and 3.4, 262144
+// (32 chunks) 4.9 and 3.0; the host saves the 2.5 us of a launch.
 constexpr int kClusterBlocks = 8;
-constexpr uint32_t kClusterChunks = 4 * kClusterBlocks;
+constexpr uint32_t kClusterChunks = 2 * kClusterBlocks;
 
 __global__ void __cluster_dims__(kClusterBlocks, 1, 1) __launch_bounds__(kThreads)
 grad_norm_small_kernel(const __grid_constant__ TensorList<kFewTensors> list, const Results out) {

@@ -18,11 +18,23 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .flash_attention import _CODES, _prepare_bias, _strides3, next_dropout_rng
+from .flash_attention import _CODES, _I64x3, _prepare_bias, next_dropout_rng
 
 _I64x2 = ctypes.c_int64 * 2
 #: buckets of one side (the C ABI passes their starts in kernel arguments)
 MAX_BUCKETS_PER_SIDE = 256
+
+
+@lru_cache(maxsize=1024)
+def _strides(strides: Tuple[int, ...]):
+    """(batch, head, row) strides of a (B, H, S, D) tensor for the C ABI, which only reads them: a model's
+    calls have few different ones."""
+    return _I64x3(*strides[:3])
+
+
+@lru_cache(maxsize=1024)
+def _table_strides(strides: Tuple[int, int]):
+    return _I64x2(*strides)
 
 
 @lru_cache(maxsize=64)
@@ -149,12 +161,13 @@ class _Call:
         if lse or self.M > 1 or self.dropout_p > 0.0:
             workspace = torch.empty(_workspace_bytes(self.H, self.M, self.N, *self.key, self.offset, rows),
                                     dtype=torch.uint8, device=self.device)
-        ts = table.stride()
         _lib.check(_lib.load().fo_rel_attn_fwd(
-            Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), lse_t.data_ptr() if lse else None, self.B, self.H, self.M, self.N, self.D,
-            _strides3(Q), _strides3(K), _strides3(V), _strides3(O), self.code, self.causal, self.scale,
-            table.data_ptr(), _I64x2(ts[0], ts[1]), self.table_code, self.starts, self.n_starts, self.bidirectional,
-            self.offset, None if workspace is None else workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
+            Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), lse_t.data_ptr() if lse else None,
+            self.B, self.H, self.M, self.N, self.D,
+            _strides(Q.stride()), _strides(K.stride()), _strides(V.stride()), _strides(O.stride()),
+            self.code, self.causal, self.scale, table.data_ptr(), _table_strides(table.stride()), self.table_code,
+            self.starts, self.n_starts, self.bidirectional, self.offset,
+            None if workspace is None else workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
             _lib.current_stream_ptr(self.index)))
         return O, lse_t, workspace
 
@@ -189,9 +202,10 @@ class _Call:
             dK.data_ptr(), dV.data_ptr(), None if dtable is None else dtable.data_ptr(), dq_accum,
             partial_sums + 4 * partials, partial_sums,
             self.B, self.H, self.M, self.N, self.D,
-            _strides3(Q), _strides3(K), _strides3(V), _strides3(O), _strides3(dO), _strides3(dQ), _strides3(dK),
-            _strides3(dV), self.code, self.causal, self.scale, self.table_code, self.starts, self.n_starts,
-            self.bidirectional, self.offset, workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
+            _strides(Q.stride()), _strides(K.stride()), _strides(V.stride()), _strides(O.stride()), _strides(dO.stride()),
+            _strides(dQ.stride()), _strides(dK.stride()), _strides(dV.stride()), self.code, self.causal,
+            self.scale, self.table_code, self.starts, self.n_starts, self.bidirectional, self.offset,
+            workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
             _lib.current_stream_ptr(self.index)))
         return dQ, dK, dV, dtable
 
