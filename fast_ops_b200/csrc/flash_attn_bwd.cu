@@ -55,8 +55,9 @@ attn_bwd_prepare_kernel(const uint16_t* __restrict__ o, const uint16_t* __restri
 }
 
 // dQ = round(dq_accum) in the input type.  One thread per 8 elements.
-// kOverlap: launched so that it may run beside the kernel before it on the stream, on which it does not depend; its
-// blocks end behind that kernel's, so that what follows on the stream waits for both.
+// kOverlap: launched so that it may run beside the kernel before it on the stream, on which it does not depend (that
+// kernel starts when the one that writes dq_accum has ended); its blocks end behind that kernel's, so that
+// what follows on the stream waits for both.
 template <bool kBf16, bool kOverlap = false>
 __global__ void __launch_bounds__(256)
 attn_bwd_finish_dq_kernel(const float* __restrict__ dq_accum, uint16_t* __restrict__ dq, int H, int Sq, int D,
@@ -72,8 +73,9 @@ attn_bwd_finish_dq_kernel(const float* __restrict__ dq_accum, uint16_t* __restri
   const int64_t bh = r / Sq;
   const int row = static_cast<int>(r - bh * Sq);
   const int b = static_cast<int>(bh / H), h = static_cast<int>(bh - static_cast<int64_t>(b) * H);
-  const float4 a0 = *reinterpret_cast<const float4*>(dq_accum + r * D + d0);
-  const float4 a1 = *reinterpret_cast<const float4*>(dq_accum + r * D + d0 + 4);
+  const float4* const src = reinterpret_cast<const float4*>(dq_accum + r * D + d0);
+  const float4 a0 = kOverlap ? __ldcg(src) : src[0];
+  const float4 a1 = kOverlap ? __ldcg(src + 1) : src[1];
   uint4 v;
   v.x = fo::pack2<kBf16>(a0.x, a0.y);
   v.y = fo::pack2<kBf16>(a0.z, a0.w);
