@@ -182,6 +182,7 @@ class Lion(Optimizer):
     @torch.no_grad()
     def step(self) -> None:
         """Parameter and momentum update (no closure, no return value: lion_optimizer.py:57)."""
+        self.grad_norm = None
         if self._zero is not None:
             self._zero.step()
             return
@@ -226,7 +227,6 @@ class Lion(Optimizer):
             grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
             self._grad_list = (lists, GradList(grads) if grads else None)
         if self._grad_list[1] is None:
-            self.grad_norm = None
             return None
         self.grad_norm, buffer = self._grad_list[1].launch(max_norm)
         return buffer

@@ -211,6 +211,17 @@ def test_clipping_options(cuda_device):
         opt.step()
 
 
+def test_no_norm_is_left_from_a_step_before_clipping_was_turned_off(cuda_device):
+    p = torch.nn.Parameter(torch.ones(10, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = Lion([p], max_grad_norm=1.0)
+    opt.step()
+    assert opt.grad_norm.item() == torch.tensor(10.0).sqrt().item()
+    opt.max_grad_norm = None
+    opt.step()
+    assert opt.grad_norm is None
+
+
 def test_a_gradient_of_infinities_does_not_pass_for_a_small_one(cuda_device):
     p = torch.nn.Parameter(torch.zeros(10, device="cuda"))
     p.grad = torch.full_like(p, 1.0)
