@@ -149,13 +149,11 @@ class Lion(Optimizer):
     # -- multi-tensor path ---------------------------------------------------------------
     @staticmethod
     def _signature(group) -> List[int]:
-        """Addresses of every parameter and of its gradient (0 = no gradient), in order: what
+        """Addresses of every parameter, then of every gradient (0 = no gradient), in order: what
         decides whether the launches prepared for this group last step can be issued again."""
-        sig = []
-        for param in group["params"]:
-            grad = param.grad
-            sig.append(param.data_ptr())
-            sig.append(0 if grad is None else grad.data_ptr())
+        params = group["params"]
+        sig = list(map(Tensor.data_ptr, params))
+        sig += [0 if (grad := param.grad) is None else grad.data_ptr() for param in params]
         return sig
 
     def _prepare_group(self, gi: int, group) -> list:
