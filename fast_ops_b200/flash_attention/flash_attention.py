@@ -16,13 +16,25 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 from .. import _lib
 
 
 _I64x3 = ctypes.c_int64 * 3
 _CODES = {torch.float16: _lib.FO_F16, torch.bfloat16: _lib.FO_BF16}
+
+
+def recorded(*tensors: Tensor) -> bool:
+    """Whether a call on these tensors goes through its autograd function: it does for a gradient, and while
+    forward-mode derivatives are taken, which the function refuses (past it a tangent would be lost without a word)."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return False
 
 
 def _strides3(t: Tensor, bshd: bool = False):
@@ -330,7 +342,7 @@ def multi_head_attention(Q: Tensor, K: Tensor, V: Tensor, *, causal: bool = Fals
     """
     if not causal and softmax_scale is None and not return_lse and bias is None and dropout_p == 0.0:
         return FlashAttentionFunction.apply(Q, K, V)
-    if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad):
+    if recorded(Q, K, V):
         return _AttentionFunction.apply(Q, K, V, bool(causal), softmax_scale, bias, float(dropout_p), None, False,
                                         return_lse)
     rng = None

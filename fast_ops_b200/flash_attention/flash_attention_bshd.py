@@ -9,10 +9,9 @@ from __future__ import annotations
 
 from typing import Optional
 
-import torch
 from torch import Tensor
 
-from .flash_attention import _AttentionFunction, _forward, dropout_mask, next_dropout_rng
+from .flash_attention import _AttentionFunction, _forward, dropout_mask, next_dropout_rng, recorded
 
 
 def flash_attn_bshd(q: Tensor, k: Tensor, v: Tensor, bias: Optional[Tensor] = None, causal: bool = False,
@@ -25,7 +24,7 @@ def flash_attn_bshd(q: Tensor, k: Tensor, v: Tensor, bias: Optional[Tensor] = No
     # (flash_attention_triton.py:780), so the offsets of later draws agree with a reference run.
     rng = next_dropout_rng(q.device, q.shape[0] * q.shape[2] * q.shape[1] * k.shape[1])
     # O has q's layout in both paths, as in the reference (flash_attention_triton.py:773)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if recorded(q, k, v):
         return _AttentionFunction.apply(q, k, v, bool(causal), softmax_scale, bias, float(dropout_p), rng, True)
     return _forward(q, k, v, True, causal, softmax_scale, False, None, bias, float(dropout_p), rng)
 

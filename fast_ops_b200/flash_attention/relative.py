@@ -18,7 +18,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .flash_attention import _CODES, _I64x3, _prepare_bias, next_dropout_rng
+from .flash_attention import _CODES, _I64x3, _prepare_bias, next_dropout_rng, recorded
 
 _I64x2 = ctypes.c_int64 * 2
 #: buckets of one side (the C ABI passes their starts in kernel arguments)
@@ -241,7 +241,7 @@ def relative_attention(Q: Tensor, K: Tensor, V: Tensor, table: Tensor, *, max_di
     """softmax(scale * Q K^T + table[bucket(j - i - query_offset)] [+ bias] [+ causal mask]) V.
 
     Q: (B, H, M, D); K, V: (B, H, N, D); fp16 or bf16, layouts as in `multi_head_attention` (K and V may
-    be expanded over the heads).  Differentiable in Q, K, V and `table`.
+    be expanded over the heads).  Differentiable in Q, K, V and `table`, once and in reverse mode.
 
     :param table: (num_buckets, H), fp32 or Q's dtype, any non-negative strides.
     :param max_distance, bidirectional: the buckets, see `relative_bucket_starts`.  Bidirectional, keys
@@ -261,10 +261,9 @@ def relative_attention(Q: Tensor, K: Tensor, V: Tensor, table: Tensor, *, max_di
     change from run to run.
     """
     call = _Call(Q, K, V, table, max_distance, bidirectional, query_offset, causal, softmax_scale, dropout_p, rng)
-    if torch.is_grad_enabled():
-        if bias is not None and bias.requires_grad:
-            raise RuntimeError("the gradient of bias is not supported (that of table is)")
-        if Q.requires_grad or K.requires_grad or V.requires_grad or table.requires_grad:
-            return _RelativeAttentionFunction.apply(Q, K, V, table, call, bias, return_lse)
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("the gradient of bias is not supported (that of table is)")
+    if recorded(Q, K, V, table):
+        return _RelativeAttentionFunction.apply(Q, K, V, table, call, bias, return_lse)
     O, lse, _ = call.forward(Q, K, V, table, bias, return_lse)
     return (O, lse) if return_lse else O
