@@ -169,15 +169,19 @@ struct Results {
   double* sumsq;
   float* norm;
   float* coef;
-  float max_norm;
+  double max_norm;
 };
 
 __device__ __forceinline__ void store_results(const Results& out, double sum) {
   if (out.sumsq != nullptr) *out.sumsq = sum;
-  const float norm = static_cast<float>(sqrt(sum));
+  const double root = sqrt(sum);
+  const float norm = static_cast<float>(root);
   if (out.norm != nullptr) *out.norm = norm;
   if (out.coef != nullptr) {
-    const float coef = __fdiv_rn(out.max_norm, __fadd_rn(norm, 1e-6f));
+    // In fp32, as clipping in memory by the norm that is reported.  Finite gradients can have a norm beyond fp32; by
+    // the infinity that is reported they would all become 0, so they are scaled by the root in double.
+    const float coef = isinf(norm) ? static_cast<float>(out.max_norm / root)
+                                   : __fdiv_rn(static_cast<float>(out.max_norm), __fadd_rn(norm, 1e-6f));
     *out.coef = coef > 1.f ? 1.f : coef;  // a NaN stays one
   }
 }
@@ -308,7 +312,7 @@ extern "C" int fo_grad_norm(const void* const* grads, const int64_t* numels, con
   fo::DeviceGuard guard(device);
   FO_REQUIRE(guard.ok, "cannot make device %d current", device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Results out{sumsq, norm, coef, static_cast<float>(max_norm)};
+  const Results out{sumsq, norm, coef, max_norm};
   if (n_tensors <= kFewTensors && total <= kClusterChunks) {
     TensorList<kFewTensors> list;
     fill_list(&list, grads, numels, dtypes, 0, n_tensors);
@@ -336,5 +340,5 @@ extern "C" int fo_grad_norm_finish(const double* sumsq, double max_norm, float* 
   if (int rc = check_max_norm(max_norm)) return rc;
   fo::DeviceGuard guard(device);
   FO_REQUIRE(guard.ok, "cannot make device %d current", device);
-  return launch_finish(sumsq, 1, Results{nullptr, norm, coef, static_cast<float>(max_norm)}, static_cast<cudaStream_t>(stream));
+  return launch_finish(sumsq, 1, Results{nullptr, norm, coef, max_norm}, static_cast<cudaStream_t>(stream));
 }

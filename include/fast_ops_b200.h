@@ -326,15 +326,17 @@ int fo_lion_flat_step_push_clipped(void* param, const void* grad, void* exp_avg_
 /*
  * The 2-norm over all elements of a list of gradients and the factor that clips them to a norm:
  *   norm = sqrt(sum_t sum_i g_t[i]^2),  coef = min(1, max_norm / (norm + 1e-6))
- * Sums are formed in double, in an order that does not change from run to run; elements of any finite
- * size count (fp32 values whose squares overflow included).  An infinite or NaN gradient gives an
- * infinite or NaN norm.  The reference has no counterpart.
+ * Eight squares of fp32 elements at a time are summed in fp32 where it holds them, everything else in double, in an
+ * order that does not change from run to run; elements of any finite size count (fp32 values whose squares
+ * overflow included).  coef is computed in fp32 from the rounded norm, or in double where the norm of finite elements
+ * is beyond fp32 (norm is then infinite).  An infinite gradient gives norm infinity and coef 0, a NaN gives NaN
+ * for both.  The reference has no counterpart.
  *
  *   grads, numels, dtypes : HOST arrays of n_tensors device pointers, element counts and element
  *                types (FO_F16, FO_BF16, FO_F32, mixed as they come); each tensor dense.  The list
  *                travels in the kernel's arguments: nothing is cached or allocated, and a call may be
  *                captured into a CUDA graph without one outside before it.
- *   max_norm   : non-negative, may be infinite (coef is then 1 unless the norm is infinite or NaN).
+ *   max_norm   : non-negative, may be infinite (coef is then 1, or NaN for an infinite or NaN gradient).
  *   workspace  : device memory of fo_grad_norm_workspace(n_tensors) doubles, 8-byte aligned, not
  *                shared with a call that may run at the same time; contents on entry do not matter.
  *   sumsq      : device double that receives the sum of squares, or NULL.
