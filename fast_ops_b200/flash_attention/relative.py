@@ -176,7 +176,8 @@ class _Call:
         """(dQ, dK, dV, the table's gradient or None)."""
         sb, sh, ss, sd = dO.stride()
         if sd != 1 or sb % 8 or sh % 8 or ss % 8 or not (sb and sh and ss) or dO.data_ptr() % 16:
-            dO = dO.contiguous()  # broadcast or cut from a larger tensor
+            # broadcast or cut from a larger tensor (where it may be dense and still begin between two 16-byte addresses)
+            dO = dO.clone(memory_format=torch.contiguous_format)
         if K.stride(1) == 0 or V.stride(1) == 0:
             # one K/V head for all query heads: one dK, dV per query head needs storage of its own
             # (autograd sums them through the expand)

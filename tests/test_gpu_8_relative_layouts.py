@@ -1,0 +1,34 @@
+"""relative_attention's gradients for layouts that a training step can meet: the same as for dense copies, bit for bit where
+the sums have a fixed order (dQ is summed by atomic adds)."""
+import pytest
+import torch
+
+from fast_ops_b200.flash_attention import relative_attention
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def same(got, want):
+    for i in (1, 2, 3):
+        assert torch.equal(got[i], want[i]), i
+    assert torch.allclose(got[0].float(), want[0].float(), rtol=2.0**-7, atol=1e-6)
+
+
+def inputs(B, H, M, N, D, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.empty(s, dtype=BF, device="cuda").normal_(generator=gen)  # noqa: E731
+    return r(B, H, M, D), r(B, H, N, D), r(B, H, N, D), r(32, H), r(B, H, M, D)
+
+
+@pytest.mark.parametrize("M", [1, 100])
+@pytest.mark.parametrize("at", [1, 4])
+def test_an_output_gradient_that_begins_between_aligned_addresses(M, at, cuda_device):
+    Q, K, V, table, dO = inputs(2, 3, M, 130, 64)
+    leaves = [t.clone().requires_grad_() for t in (Q, K, V, table)]
+    O = relative_attention(*leaves)
+    flat = torch.zeros(dO.numel() + 8, dtype=BF, device="cuda")
+    g = flat[at:at + dO.numel()].view(dO.shape)
+    g.copy_(dO)
+    assert g.is_contiguous() and g.data_ptr() % 16
+    same(torch.autograd.grad(O, leaves, g, retain_graph=True), torch.autograd.grad(O, leaves, dO))
