@@ -85,9 +85,11 @@ attn_bwd_finish_dq_kernel(const float* __restrict__ dq_accum, uint16_t* __restri
   if constexpr (kOverlap) fo::grid_wait_previous();
 }
 
-int check_out_strides(const int64_t s[3], const char* name) {
+// (A dimension of extent 1 never uses its stride.)
+int check_out_strides(const int64_t s[3], int B, int H, int S, const char* name) {
+  const int extent[3] = {B, H, S};
   for (int i = 0; i < 3; ++i)
-    FO_REQUIRE(s[i] >= 0 && s[i] % 8 == 0, "%s: strides must be non-negative multiples of 8 elements", name);
+    FO_REQUIRE(extent[i] == 1 || (s[i] >= 0 && s[i] % 8 == 0), "%s: strides must be non-negative multiples of 8 elements", name);
   return FO_OK;
 }
 
@@ -116,10 +118,10 @@ int fo::attn_bwd_impl(const void* q, const void* k, const void* v, const void* o
                         static_cast<const void*>(dv)})
     FO_REQUIRE((reinterpret_cast<uintptr_t>(p) & 15) == 0, "o, dq, dk, dv must be 16-byte aligned");
   FO_REQUIRE((reinterpret_cast<uintptr_t>(dq_accum) & 15) == 0, "dq_accum must be 16-byte aligned");
-  if (int rc = check_out_strides(o_strides, "o")) return rc;
-  if (int rc = check_out_strides(dq_strides, "dq")) return rc;
-  if (int rc = check_out_strides(dk_strides, "dk")) return rc;
-  if (int rc = check_out_strides(dv_strides, "dv")) return rc;
+  if (int rc = check_out_strides(o_strides, B, H, Sq, "o")) return rc;
+  if (int rc = check_out_strides(dq_strides, B, H, Sq, "dq")) return rc;
+  if (int rc = check_out_strides(dk_strides, B, H, Sk, "dk")) return rc;
+  if (int rc = check_out_strides(dv_strides, B, H, Sk, "dv")) return rc;
 
   fo::DeviceGuard guard(device);
   FO_REQUIRE(guard.ok, "cannot make device %d current", device);

@@ -3,7 +3,7 @@ the sums have a fixed order (dQ is summed by atomic adds)."""
 import pytest
 import torch
 
-from fast_ops_b200.flash_attention import relative_attention
+from fast_ops_b200.flash_attention import multi_head_attention, relative_attention
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -32,3 +32,18 @@ def test_an_output_gradient_that_begins_between_aligned_addresses(M, at, cuda_de
     g.copy_(dO)
     assert g.is_contiguous() and g.data_ptr() % 16
     same(torch.autograd.grad(O, leaves, g, retain_graph=True), torch.autograd.grad(O, leaves, dO))
+
+
+@pytest.mark.parametrize("M,N", [(1, 130), (70, 1), (1, 1)])
+def test_rows_of_stride_one_where_there_is_one_row(M, N, cuda_device):
+    """(B, H, D, 1) tensors transposed: the gradients of Q or of K and V get the same strides."""
+    Q, K, V, table, dO = inputs(2, 3, M, N, 64)
+    want_leaves = [t.clone().requires_grad_() for t in (Q, K, V, table)]
+    want = torch.autograd.grad(relative_attention(*want_leaves), want_leaves, dO)
+    column = lambda t: t.clone().view(2, 3, 64, 1).transpose(2, 3) if t.shape[2] == 1 else t.clone()  # noqa: E731
+    leaves = [column(t).requires_grad_() for t in (Q, K, V)] + [table.clone().requires_grad_()]
+    assert any(t.stride(2) == 1 for t in leaves[:3])
+    same(torch.autograd.grad(relative_attention(*leaves), leaves, dO), want)
+    plain = torch.autograd.grad(multi_head_attention(*leaves[:3]), leaves[:3], dO)
+    dense = torch.autograd.grad(multi_head_attention(*want_leaves[:3]), want_leaves[:3], dO)
+    same(plain + (table,), dense + (table,))

@@ -73,3 +73,28 @@ def test_output_gradients_reach_the_library_in_a_layout_that_it_takes(shape, mon
             assert extent == 1 or (stride > 0 and stride % 8 == 0), name
         assert torch.equal(record.dO, dO), name
         monkeypatch.undo()
+
+
+@pytest.mark.parametrize("entry", ["fo_rel_attn_bwd", "fo_flash_attn_bwd"])
+def test_a_dimension_of_extent_1_may_have_any_stride(entry):
+    """A (B, H, D, 1) tensor transposed to (B, H, 1, D) has row stride 1, and so has a gradient made like it.  (dv's strides
+    are wrong on purpose: they are checked behind the others, and before any CUDA call.)"""
+    lib = L.load()
+    i3 = ctypes.c_int64 * 3
+    one, rows, wrong = i3(2 * 64, 64, 1), i3(8 * 64 * 2, 8 * 64, 64), i3(8 * 64 * 2, 8 * 64, 63)
+
+    def call(o, dq, dk, dv, H=2, Sq=1):
+        if entry == "fo_rel_attn_bwd":
+            starts = (ctypes.c_int * 2)(0, 1)
+            lib.fo_rel_attn_bwd(*([16] * 9), None, 16, 16, None, 1, H, Sq, 8, 64, one, rows, rows, o, one, dq, dk, dv,
+                                L.FO_BF16, 0, 0.125, L.FO_F32, starts, 2, 1, 0, 16, None, None, L.FO_F32, 0.0, 0, 0, 0, None)
+        else:
+            lib.fo_flash_attn_bwd(*([16] * 11), 1, H, Sq, 8, 64, one, rows, rows, o, one, dq, dk, dv, L.FO_BF16, 0, 0.125, 0, None)
+        return lib.fo_last_error()
+
+    assert call(one, one, rows, wrong).startswith(b"dv: strides")
+    assert call(i3(3, 64, 1), i3(5, 64, 7), i3(7, 8 * 64, 64), wrong).startswith(b"dv: strides")  # a batch of one too
+    assert call(one, one, rows, wrong, Sq=2).startswith(b"o: strides")
+    assert call(rows, one, rows, wrong, Sq=2).startswith(b"dq: strides")
+    assert call(one, one, wrong, rows).startswith(b"dk: strides")
+    assert call(one, i3(128, 4, 1), rows, wrong, H=1).startswith(b"dv: strides")
