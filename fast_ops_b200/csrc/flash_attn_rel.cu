@@ -33,7 +33,7 @@ struct ExpandParams {
   int bias_f32;
   int bias_heads;       // heads of the rows made of it
   float inv_scale;      // 1 / softmax scale
-  int H, Sk, zero, width, stride, value_blocks, vec_width;
+  int Sk, zero, width, stride, value_blocks, vec_width;
   float* values;
   int* bucket_of;
   float* vec;
@@ -217,16 +217,10 @@ rel_table_grad_kernel(const RelBias rel, T* __restrict__ dtable, int B, int H, i
   cluster.sync();  // no block leaves while its shared memory is being read
 }
 
-// Checks of the relative bias's own arguments; fills everything of `rel` but the device pointers of the
-// expanded vector.
-int make_rel_args(RelArgs* rel, int H, int Sq, int Sk, const void* table, int table_dtype, const int64_t* table_strides,
-                  const int* starts, int n_starts, int two_sided, int query_offset, int dtype) {
-  FO_REQUIRE(dtype == FO_F16 || dtype == FO_BF16, "attention inputs must be fp16 or bf16 (got dtype %d)", dtype);
-  FO_REQUIRE(table && table_strides && starts, "null relative bias argument");
-  FO_REQUIRE(table_dtype == FO_F32 || table_dtype == dtype, "the table must be fp32 or have the dtype of q (got dtype %d)",
-             table_dtype);
-  FO_REQUIRE(reinterpret_cast<uintptr_t>(table) % (table_dtype == FO_F32 ? 4 : 2) == 0, "the table is not aligned to its elements");
-  FO_REQUIRE(table_strides[0] >= 0 && table_strides[1] >= 0, "the table's strides must be non-negative");
+// Checks of the buckets and of where the queries stand; fills everything of `rel` but the table and the device
+// pointers of the expanded vector.
+int make_rel_args(RelArgs* rel, int H, int Sq, int Sk, const int* starts, int n_starts, int two_sided, int query_offset) {
+  FO_REQUIRE(starts, "null bucket starts");
   FO_REQUIRE(n_starts >= 1 && n_starts <= fo::kRelMaxStarts, "1 to %d buckets per side (got %d)", fo::kRelMaxStarts, n_starts);
   FO_REQUIRE(starts[0] == 0, "the first bucket must start at distance 0");
   for (int i = 1; i < n_starts; ++i) FO_REQUIRE(starts[i] >= starts[i - 1], "bucket starts must not descend");
@@ -236,10 +230,6 @@ int make_rel_args(RelArgs* rel, int H, int Sq, int Sk, const void* table, int ta
   std::copy(starts, starts + n_starts, rel->buckets.starts);
   rel->buckets.n = n_starts;
   rel->buckets.two_sided = two_sided ? 1 : 0;
-  rel->table = table;
-  rel->stride_bucket = table_strides[0];
-  rel->stride_head = table_strides[1];
-  rel->table_f32 = table_dtype == FO_F32;
   RelBias& bias = rel->bias;
   bias.offset = query_offset;
   bias.num_buckets = n_starts * (two_sided ? 2 : 1);
@@ -254,6 +244,26 @@ int make_rel_args(RelArgs* rel, int H, int Sq, int Sk, const void* table, int ta
   return FO_OK;
 }
 
+// The type that the table or its gradient has.
+int check_table_dtype(int table_dtype, int dtype) {
+  FO_REQUIRE(dtype == FO_F16 || dtype == FO_BF16, "attention inputs must be fp16 or bf16 (got dtype %d)", dtype);
+  FO_REQUIRE(table_dtype == FO_F32 || table_dtype == dtype, "the table must be fp32 or have the dtype of q (got dtype %d)",
+             table_dtype);
+  return FO_OK;
+}
+
+int set_table(RelArgs* rel, const void* table, int table_dtype, const int64_t* table_strides, int dtype) {
+  FO_REQUIRE(table && table_strides, "null relative bias argument");
+  if (int rc = check_table_dtype(table_dtype, dtype)) return rc;
+  FO_REQUIRE(reinterpret_cast<uintptr_t>(table) % (table_dtype == FO_F32 ? 4 : 2) == 0, "the table is not aligned to its elements");
+  FO_REQUIRE(table_strides[0] >= 0 && table_strides[1] >= 0, "the table's strides must be non-negative");
+  rel->table = table;
+  rel->stride_bucket = table_strides[0];
+  rel->stride_head = table_strides[1];
+  rel->table_f32 = table_dtype == FO_F32;
+  return FO_OK;
+}
+
 // The expanded bias in a workspace: values, rows of the vector bias, buckets.
 int64_t expanded_bytes(const RelBias& bias, int H, int64_t bias_rows, int Sk) {
   const int64_t width = fo::rel_vec_width(Sk);
@@ -262,7 +272,8 @@ int64_t expanded_bytes(const RelBias& bias, int H, int64_t bias_rows, int Sk) {
 
 int set_expanded(RelArgs* rel, void* workspace, const fo::AttnExtras& ex, int B, int H, int Sk, bool needed) {
   if (!needed) return FO_OK;
-  FO_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be given, 16-byte aligned");
+  FO_REQUIRE(workspace != nullptr, "null workspace");
+  FO_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "workspace must be 16-byte aligned");
   FO_REQUIRE(B > 0 && H > 0, "B and H must be positive (got %d %d)", B, H);
   RelBias& bias = rel->bias;
   bias.values = static_cast<const float*>(workspace);
@@ -324,7 +335,6 @@ int launch_rel_expand(const RelArgs& rel, const AttnExtras& ex, int H, int Sk, f
   prm.bias_f32 = ex.bias_f32;
   prm.bias_heads = rel.bias_heads;
   prm.inv_scale = 1.f / softmax_scale;
-  prm.H = H;
   prm.Sk = Sk;
   prm.zero = rel.bias.zero;
   prm.width = rel.bias.width;
@@ -420,9 +430,7 @@ extern "C" int64_t fo_rel_attn_workspace(int H, int Sq, int Sk, const int* start
                                          int query_offset, int64_t bias_rows) {
   fo::clear_error();
   RelArgs rel;
-  const int64_t strides[2] = {0, 0};
-  const float table = 0;
-  if (make_rel_args(&rel, H, Sq, Sk, &table, FO_F32, strides, starts, n_starts, two_sided, query_offset, FO_BF16)) return -1;
+  if (make_rel_args(&rel, H, Sq, Sk, starts, n_starts, two_sided, query_offset)) return -1;
   if (H <= 0 || bias_rows < 0) {
     fo::fail(FO_ERR_INVALID_ARGUMENT, "H must be positive and bias_rows not negative (got %d %lld)", H, (long long)bias_rows);
     return -1;
@@ -451,8 +459,8 @@ extern "C" int fo_rel_attn_fwd(const void* q, const void* k, const void* v, void
                                int device, void* stream) {
   fo::clear_error();
   RelArgs rel;
-  if (int rc = make_rel_args(&rel, H, Sq, Sk, table, table_dtype, table_strides, starts, n_starts, two_sided, query_offset, dtype))
-    return rc;
+  if (int rc = make_rel_args(&rel, H, Sq, Sk, starts, n_starts, two_sided, query_offset)) return rc;
+  if (int rc = set_table(&rel, table, table_dtype, table_strides, dtype)) return rc;
   if (int rc = check_bias_strides(bias, bias_strides)) return rc;
   fo::AttnExtras ex;
   if (int rc = fo::make_attn_extras(&ex, bias, bias_strides, bias_dtype, dtype, dropout_p, rng_seed, rng_offset)) return rc;
@@ -475,10 +483,9 @@ extern "C" int fo_rel_attn_bwd(const void* q, const void* k, const void* v, cons
                                int device, void* stream) {
   fo::clear_error();
   RelArgs rel;
-  const int64_t no_strides[2] = {0, 0};
-  // the table itself is not read again: its expanded form is
-  if (int rc = make_rel_args(&rel, H, Sq, Sk, workspace, table_dtype, no_strides, starts, n_starts, two_sided, query_offset, dtype))
-    return rc;
+  // the table itself is not read again: its expanded form, in the workspace, is
+  if (int rc = make_rel_args(&rel, H, Sq, Sk, starts, n_starts, two_sided, query_offset)) return rc;
+  if (int rc = check_table_dtype(table_dtype, dtype)) return rc;
   FO_REQUIRE(dtable == nullptr || partials != nullptr, "the table's gradient needs its workspace");
   FO_REQUIRE((reinterpret_cast<uintptr_t>(partials) & 7) == 0, "partials must be 8-byte aligned");
   FO_REQUIRE(reinterpret_cast<uintptr_t>(dtable) % (table_dtype == FO_F32 ? 4 : 2) == 0, "dtable is not aligned to its elements");
