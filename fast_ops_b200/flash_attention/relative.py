@@ -156,7 +156,9 @@ class _Call:
         """(O, LSE or None, the expanded bias or None where nothing reads it)."""
         O = torch.empty_like(Q, memory_format=torch.contiguous_format)
         lse_t = Q.new_empty((self.B, self.H, self.M), dtype=torch.float32) if lse else None
-        kept, rows, bias_args = self.bias(bias, Q)
+        # Kept for the backward, which takes from the strides where in the workspace the rows of the bias lie; the saved
+        # tensors may come back with other strides than they left with (saved_tensors_hooks, save_on_cpu).
+        self.kept_bias, rows, self.bias_args = self.bias(bias, Q)
         workspace = None
         if lse or self.M > 1 or self.dropout_p > 0.0:
             workspace = torch.empty(_workspace_bytes(self.H, self.M, self.N, *self.key, self.offset, rows),
@@ -167,13 +169,13 @@ class _Call:
             _strides(Q.stride()), _strides(K.stride()), _strides(V.stride()), _strides(O.stride()),
             self.code, self.causal, self.scale, table.data_ptr(), _table_strides(table.stride()), self.table_code,
             self.starts, self.n_starts, self.bidirectional, self.offset,
-            None if workspace is None else workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
+            None if workspace is None else workspace.data_ptr(), *self.bias_args, self.dropout_p, *self.rng, self.index,
             _lib.current_stream_ptr(self.index)))
         return O, lse_t, workspace
 
     def backward(self, dO: Tensor, Q: Tensor, K: Tensor, V: Tensor, O: Tensor, LSE: Tensor, workspace: Tensor,
-                 bias: Optional[Tensor], table_grad: Optional[torch.dtype]):
-        """(dQ, dK, dV, the table's gradient or None)."""
+                 table_grad: Optional[torch.dtype]):
+        """(dQ, dK, dV, the table's gradient or None), after `forward`."""
         sb, sh, ss, sd = dO.stride()
         if sd != 1 or sb % 8 or sh % 8 or ss % 8 or not (sb and sh and ss) or dO.data_ptr() % 16:
             # broadcast or cut from a larger tensor (where it may be dense and still begin between two 16-byte addresses)
@@ -197,7 +199,6 @@ class _Call:
         scratch = torch.empty(rows * (self.D + 1) + partials, dtype=torch.float32, device=self.device)
         dq_accum = scratch.data_ptr()
         partial_sums = dq_accum + 4 * rows * self.D  # a multiple of 32 bytes on, since D is one of 8
-        kept, _, bias_args = self.bias(bias, Q)
         _lib.check(lib.fo_rel_attn_bwd(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(), dO.data_ptr(), LSE.data_ptr(), dQ.data_ptr(),
             dK.data_ptr(), dV.data_ptr(), None if dtable is None else dtable.data_ptr(), dq_accum,
@@ -206,7 +207,7 @@ class _Call:
             _strides(Q.stride()), _strides(K.stride()), _strides(V.stride()), _strides(O.stride()), _strides(dO.stride()),
             _strides(dQ.stride()), _strides(dK.stride()), _strides(dV.stride()), self.code, self.causal,
             self.scale, self.table_code, self.starts, self.n_starts, self.bidirectional, self.offset,
-            workspace.data_ptr(), *bias_args, self.dropout_p, *self.rng, self.index,
+            workspace.data_ptr(), *self.bias_args, self.dropout_p, *self.rng, self.index,
             _lib.current_stream_ptr(self.index)))
         return dQ, dK, dV, dtable
 
@@ -216,7 +217,7 @@ class _RelativeAttentionFunction(Function):
     def forward(ctx, Q: Tensor, K: Tensor, V: Tensor, table: Tensor, call: _Call, bias: Optional[Tensor],
                 return_lse: bool):
         O, lse, workspace = call.forward(Q, K, V, table, bias, True)
-        ctx.save_for_backward(Q, K, V, O, lse, workspace, bias)
+        ctx.save_for_backward(Q, K, V, O, lse, workspace)
         ctx.call, ctx.table_dtype = call, table.dtype
         if not return_lse:
             return O
@@ -229,8 +230,8 @@ class _RelativeAttentionFunction(Function):
     def backward(ctx, dO: Optional[Tensor], _dlse=None):
         if dO is None:
             return (None,) * 7
-        Q, K, V, O, lse, workspace, bias = ctx.saved_tensors
-        return ctx.call.backward(dO, Q, K, V, O, lse, workspace, bias,
+        Q, K, V, O, lse, workspace = ctx.saved_tensors
+        return ctx.call.backward(dO, Q, K, V, O, lse, workspace,
                                  ctx.table_dtype if ctx.needs_input_grad[3] else None) + (None,) * 3
 
 

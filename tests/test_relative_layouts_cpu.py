@@ -32,9 +32,9 @@ def backward(monkeypatch, dO, Q, K, V):
     call.B, call.H, call.M, call.D = Q.shape
     call.N, call.device, call.code, call.causal, call.scale = K.shape[2], Q.device, L.FO_BF16, 0, 0.125
     call.table_code, call.starts, call.n_starts, call.bidirectional, call.offset = L.FO_F32, None, 0, 1, 0
-    call.dropout_p, call.rng, call.index = 0.0, (0, 0), 0
+    call.dropout_p, call.rng, call.index, call.bias_args = 0.0, (0, 0), 0, (None, None, L.FO_F32)
     O = torch.zeros(Q.shape, dtype=BF)
-    return call.backward(dO, Q, K, V, O, torch.zeros(Q.shape[:3]), torch.zeros(16), None, None)[:3], rec
+    return call.backward(dO, Q, K, V, O, torch.zeros(Q.shape[:3]), torch.zeros(16), None)[:3], rec
 
 
 def tensor_at(ptr, shape, strides):
