@@ -23,7 +23,10 @@ Keyword-only extensions:
                    ranks' slices with process_group) and applies every gradient times
                    min(1, max_grad_norm / (norm + 1e-6)), rounded to the gradient's type once, as if
                    it had been clipped in memory.  The factor stays on the device and the stored
-                   gradients are left as they are.  `grad_norm` is the norm of the latest step.
+                   gradients are left as they are.  `grad_norm` is the norm of the latest step.  A NaN
+                   among the gradients makes the factor NaN, an infinity makes it 0 (finite gradients
+                   vanish, infinite ones give NaN); finite gradients whose norm is beyond fp32 are
+                   scaled by that norm, though `grad_norm` is infinite.
 """
 from __future__ import annotations
 
@@ -41,13 +44,6 @@ from .grad_norm import GradList, finish_norm, is_dense as _is_dense, shard_sumsq
 from .zero1 import FlatLayout
 
 _dtype_of = attrgetter("dtype")
-
-
-def _addresses(tensors: List[Optional[Tensor]]) -> List[int]:
-    try:
-        return list(map(Tensor.data_ptr, tensors))
-    except TypeError:  # some are None
-        return [0 if t is None else t.data_ptr() for t in tensors]
 
 
 def lion_update(param: Tensor, grad: Tensor, exp_avg: Tensor, lr: float, beta1: float, beta2: float,
@@ -142,8 +138,7 @@ class Lion(Optimizer):
         defaults = {"lr": lr, "betas": betas, "weight_decay": weight_decay}
         super().__init__(params, defaults)
         self._momentum_dtype = momentum_dtype
-        self._lists: Dict[int, tuple] = {}  # group index -> (parameters, signature, prepared launches)
-        self._kept: Optional[tuple] = None  # the state's parameters, momentum tensors and their addresses then
+        self._kept: Optional[tuple] = None  # (signature, prepared launches of each group, what the signature has ids of)
         self.max_grad_norm = max_grad_norm
         #: 0-d fp32 tensor: the norm of all gradients at the latest step, before clipping.  None before the
         #: first step, without max_grad_norm, and after a step in which no parameter had a gradient
@@ -162,51 +157,38 @@ class Lion(Optimizer):
     # A training loop presents the same tensors step after step, so the checks and the pointer arrays of a step
     # stand for the next one.  They hold raw addresses, and an address alone says little: a view, or memory that the
     # allocator has given to another tensor, can have the one of the step before.  So a step first compares what they
-    # were made from with the tensors it has now (0.5 us per parameter in all; new lists take 3 to 4).
-    @staticmethod
-    def _signature(params: List[Tensor]) -> list:
-        """Address, size and type of each parameter, address (0 = none) and strides of its gradient, whose type and
-        shape are the parameter's (assigning another gradient raises)."""
+    # were made from with the tensors it has now (0.4 us per parameter; new lists take 3 to 4).
+    def _signature(self) -> list:
+        """What the launches of a step are made from, column by column: the parameters of each group with their
+        addresses, sizes and types; the addresses (0 = none) and strides of their gradients, which have the
+        parameters' types and shapes (assigning others raises); the state's momentum tensors and their addresses."""
+        groups = self.param_groups
+        params = groups[0]["params"] if len(groups) == 1 else [p for group in groups for p in group["params"]]
         grads = [p.grad for p in params]
         try:
-            ptrs, strides = list(map(Tensor.data_ptr, grads)), list(map(Tensor.stride, grads))
-        except TypeError:  # some are None
-            ptrs, strides = _addresses(grads), [g if g is None else g.stride() for g in grads]
-        return [list(map(Tensor.data_ptr, params)), list(map(Tensor.numel, params)), list(map(_dtype_of, params)),
-                ptrs, strides]
+            momenta = list(map(dict.get, self.state.values(), repeat("exp_avg")))
+            optional = [list(map(Tensor.data_ptr, grads)), list(map(Tensor.stride, grads)), list(map(Tensor.data_ptr, momenta))]
+        except TypeError:  # a parameter without a gradient or a momentum, or something of the caller's own in the state
+            momenta = self._momenta()
+            optional = [[t if t is None else t.data_ptr() for t in grads], [t if t is None else t.stride() for t in grads],
+                        [t if t is None else t.data_ptr() for t in momenta]]
+        return [list(map(id, params)), list(map(Tensor.data_ptr, params)), list(map(Tensor.numel, params)),
+                list(map(_dtype_of, params)), *optional, list(map(id, self.state)), list(map(id, momenta)),
+                [len(group["params"]) for group in groups]]
 
     def _momenta(self) -> list:
-        """The momentum tensors of all parameters that have one, in the order of the state."""
-        try:
-            return list(map(dict.get, self.state.values(), repeat("exp_avg")))
-        except TypeError:  # a caller keeps something of its own in the state
-            return [s.get("exp_avg") if isinstance(s, dict) else None for s in self.state.values()]
-
-    def _momenta_stand(self) -> bool:
-        """Whether the state's momentum tensors are those of the prepared launches, at their addresses."""
-        if self._kept is None:
-            return False
-        owners, momenta, ptrs = self._kept
-        return (len(self.state) == len(owners) and all(map(is_, self.state, owners))
-                and all(map(is_, self._momenta(), momenta)) and _addresses(momenta) == ptrs)
+        """The momentum tensors of all parameters, in the order of the state; None where there is none."""
+        return [s.get("exp_avg") if isinstance(s, dict) else None for s in self.state.values()]
 
     def _prepared(self) -> List[list]:
-        """The launches of each group, those of the step before where all that they hold still stands."""
-        if not self._momenta_stand():
-            self._lists.clear()
-        fresh = False
-        for gi, group in enumerate(self.param_groups):
-            params = group["params"]
-            sig = self._signature(params)
-            cached = self._lists.pop(gi, None)
-            if cached is None or len(cached[0]) != len(params) or not all(map(is_, cached[0], params)) or cached[1] != sig:
-                fresh = True
-                cached = (list(params), sig, self._prepare_group(gi, group))
-            self._lists[gi] = cached
-        if fresh:  # the references keep the momentum's memory from being given to another tensor
-            momenta = self._momenta()
-            self._kept = (list(self.state), momenta, _addresses(momenta))
-        return [self._lists[gi][2] for gi in range(len(self.param_groups))]
+        """The launches of each group: those of the step before where they stand."""
+        if self._kept is None or self._kept[0] != self._signature():
+            self._kept = None
+            lists = [self._prepare_group(gi, group) for gi, group in enumerate(self.param_groups)]
+            # (the references keep an id, or a momentum's memory, from being given to another tensor)
+            self._kept = (self._signature(), lists,
+                          [p for group in self.param_groups for p in group["params"]], list(self.state), self._momenta())
+        return self._kept[1]
 
     def _prepare_group(self, gi: int, group) -> list:
         """Checks every (param, grad, exp_avg) triple of the group, creates missing momentum, and
@@ -279,8 +261,7 @@ class Lion(Optimizer):
         """As torch.optim.Optimizer.load_state_dict; in process_group mode the loaded momentum
         (this rank's slices, as state_dict() saved them) is copied back into the rank's shard."""
         super().load_state_dict(state_dict)
-        self._lists.clear()  # the momentum tensors are new objects
-        self._kept = self._grad_list = None
+        self._kept = self._grad_list = None  # the momentum tensors are new objects
         if self._zero is not None:
             self._zero.adopt_loaded_state()
 
