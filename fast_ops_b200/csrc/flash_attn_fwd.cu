@@ -361,9 +361,9 @@ int fo::attn_fwd_impl(const void* q, const void* k, const void* v, void* o, floa
   const bool bf16 = dtype == FO_BF16;
   if (rel) {
     if (int rc = fo::launch_rel_expand(*rel, *ex, H, Sk, softmax_scale, bf16, s)) return rc;
-    // One query tile per CTA: the faster one at every shape measured (us, it and the paired kernel: B1 H16 S8192
-    // D128 causal 288 and 304, S16384 1155 and 1149; B2 H16 S4096 D128 157 and 173, padded 175 and 203; B8 H12
-    // S1024 D64 61 and 69).  It keeps the bias vector in shared memory, so buckets that reach too far (about 860
+    // One query tile per CTA: the faster one up to 8192 keys, and within 1 % at 16384 (us, it and the paired kernel:
+    // B1 H16 S8192 D128 causal 288 and 304, S16384 1155 and 1149; B2 H16 S4096 D128 157 and 173, padded 175 and 203;
+    // B8 H12 S1024 D64 61 and 69).  It keeps the bias vector in shared memory, so buckets that reach too far (about 860
     // two-sided at head_dim 128, 1880 at 64) take the paired kernel, and so does dropout.
     prm.rel.smem_copies = Dk == 64 ? fo::Ws64sConfig<64>::rel_copies(prm.rel.stride) : fo::Ws64sConfig<128>::rel_copies(prm.rel.stride);
     const bool half_tiles = !ex->dropout && prm.rel.smem_copies != 0 && impl != AttnImpl::kWarpSpecialized64;

@@ -245,7 +245,8 @@ def relative_attention(Q: Tensor, K: Tensor, V: Tensor, table: Tensor, *, max_di
     Q: (B, H, M, D); K, V: (B, H, N, D); fp16 or bf16, layouts as in `multi_head_attention` (K and V may
     be expanded over the heads).  Differentiable in Q, K, V and `table`, once and in reverse mode.
 
-    :param table: (num_buckets, H), fp32 or Q's dtype, any non-negative strides.
+    :param table: (num_buckets, H), fp32 or Q's dtype, any non-negative strides; entries of -1e6 and below
+        mask the keys of their bucket, as -inf does.
     :param max_distance, bidirectional: the buckets, see `relative_bucket_starts`.  Bidirectional, keys
         before and after the query have num_buckets / 2 buckets each; otherwise all buckets are for the
         keys before it and those after it are at distance 0 (as a causal model wants it).
@@ -260,7 +261,9 @@ def relative_attention(Q: Tensor, K: Tensor, V: Tensor, table: Tensor, *, max_di
     :returns: O (B, H, M, D), contiguous, or (O, LSE) with `return_lse`.
 
     Violations of these raise RuntimeError.  The table's gradient is summed in an order that does not
-    change from run to run.
+    change from run to run.  P and dS are rounded to Q's dtype for their matmuls, as in the framework's other
+    attention calls; everything else is fp32 or wider.  While a backward runs it holds scratch for the
+    table's gradient that grows with M N: 4 to 8 bytes for every 32 x 32 scores (fo_rel_attn_bwd_workspace).
     """
     call = _Call(Q, K, V, table, max_distance, bidirectional, query_offset, causal, softmax_scale, dropout_p, rng)
     if bias is not None and bias.requires_grad and torch.is_grad_enabled():

@@ -94,10 +94,11 @@ def grad_norm(grads: Iterable[Tensor]) -> Tensor:
     """The 2-norm of all elements of `grads` together, a 0-d fp32 tensor on their device.
 
     The tensors may be fp16, bf16 and fp32, mixed as they come, of any size, each dense in memory and
-    all on one CUDA device (violations raise RuntimeError, an empty list too).  Sums are formed in
-    double in a fixed order: the same gradients give the same bits, and squares that leave the range
-    of fp32 count.  Non-finite gradients give a non-finite norm.  Not differentiable.  The call
-    does not wait for the device and may be captured into a CUDA graph.
+    all on one CUDA device (violations raise RuntimeError, an empty list too).  The squares of eight fp32
+    elements at a time are summed in fp32 where it holds them, everything else in double, in a fixed
+    order: the same gradients give the same bits, and squares that leave the range of fp32 count.  A
+    norm beyond fp32 is infinite, non-finite gradients give a non-finite norm.  Not differentiable.  The
+    call does not wait for the device and may be captured into a CUDA graph.
     """
     if isinstance(grads, Tensor):
         grads = [grads]
