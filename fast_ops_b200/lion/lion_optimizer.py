@@ -32,8 +32,9 @@ from __future__ import annotations
 
 import ctypes
 from itertools import repeat
-from operator import attrgetter, is_
+from operator import attrgetter, call, is_
 from typing import Dict, Iterable, List, Optional, Tuple
+from weakref import ref
 
 import torch
 from torch import Tensor
@@ -138,7 +139,7 @@ class Lion(Optimizer):
         defaults = {"lr": lr, "betas": betas, "weight_decay": weight_decay}
         super().__init__(params, defaults)
         self._momentum_dtype = momentum_dtype
-        self._kept: Optional[tuple] = None  # (signature, prepared launches of each group, what the signature has ids of)
+        self._kept: Optional[tuple] = None  # what _prepared made for the step before
         self.max_grad_norm = max_grad_norm
         #: 0-d fp32 tensor: the norm of all gradients at the latest step, before clipping.  None before the
         #: first step, without max_grad_norm, and after a step in which no parameter had a gradient
@@ -158,10 +159,11 @@ class Lion(Optimizer):
     # stand for the next one.  They hold raw addresses, and an address alone says little: a view, or memory that the
     # allocator has given to another tensor, can have the one of the step before.  So a step first compares what they
     # were made from with the tensors it has now (0.4 us per parameter; new lists take 3 to 4).
-    def _signature(self) -> list:
+    def _signature(self) -> Tuple[list, list]:
         """What the launches of a step are made from, column by column: the parameters of each group with their
-        addresses, sizes and types; the addresses (0 = none) and strides of their gradients, which have the
-        parameters' types and shapes (assigning others raises); the state's momentum tensors and their addresses."""
+        addresses, sizes and types; the addresses (None: no gradient) and strides of their gradients, which have the
+        parameters' types and shapes (assigning others raises); the state's keys and its momentum tensors' addresses.
+        Beside it the momentum tensors themselves, in the order of the state (None where there is none)."""
         groups = self.param_groups
         params = groups[0]["params"] if len(groups) == 1 else [p for group in groups for p in group["params"]]
         grads = [p.grad for p in params]
@@ -169,26 +171,28 @@ class Lion(Optimizer):
             momenta = list(map(dict.get, self.state.values(), repeat("exp_avg")))
             optional = [list(map(Tensor.data_ptr, grads)), list(map(Tensor.stride, grads)), list(map(Tensor.data_ptr, momenta))]
         except TypeError:  # a parameter without a gradient or a momentum, or something of the caller's own in the state
-            momenta = self._momenta()
+            momenta = [s.get("exp_avg") if isinstance(s, dict) else None for s in self.state.values()]
             optional = [[t if t is None else t.data_ptr() for t in grads], [t if t is None else t.stride() for t in grads],
                         [t if t is None else t.data_ptr() for t in momenta]]
         return [list(map(id, params)), list(map(Tensor.data_ptr, params)), list(map(Tensor.numel, params)),
-                list(map(_dtype_of, params)), *optional, list(map(id, self.state)), list(map(id, momenta)),
-                [len(group["params"]) for group in groups]]
-
-    def _momenta(self) -> list:
-        """The momentum tensors of all parameters, in the order of the state; None where there is none."""
-        return [s.get("exp_avg") if isinstance(s, dict) else None for s in self.state.values()]
+                list(map(_dtype_of, params)), *optional, list(map(id, self.state)),
+                [len(group["params"]) for group in groups]], momenta
 
     def _prepared(self) -> List[list]:
         """The launches of each group: those of the step before where they stand."""
-        if self._kept is None or self._kept[0] != self._signature():
-            self._kept = None
-            lists = [self._prepare_group(gi, group) for gi, group in enumerate(self.param_groups)]
-            # (the references keep an id, or a momentum's memory, from being given to another tensor)
-            self._kept = (self._signature(), lists,
-                          [p for group in self.param_groups for p in group["params"]], list(self.state), self._momenta())
-        return self._kept[1]
+        kept = self._kept
+        if kept is not None:
+            signature, momenta = self._signature()
+            if kept[0] == signature and all(map(is_, map(call, kept[2]), momenta)):
+                return kept[1]
+        self._kept = None
+        lists = [self._prepare_group(gi, group) for gi, group in enumerate(self.param_groups)]
+        signature, momenta = self._signature()
+        # A momentum tensor that the caller takes out of the state is to be freed, so it is held weakly; the
+        # parameters and keys are held, so that their ids are not given to others.
+        self._kept = (signature, lists, [type(None) if m is None else ref(m) for m in momenta],
+                      [p for group in self.param_groups for p in group["params"]], list(self.state))
+        return lists
 
     def _prepare_group(self, gi: int, group) -> list:
         """Checks every (param, grad, exp_avg) triple of the group, creates missing momentum, and

@@ -1,6 +1,8 @@
 """The launches that a Lion step keeps for the next one, without a GPU: whatever they hold of a parameter, a
 gradient or a momentum tensor is compared with the tensors of the step that issues them again.  The device calls are
 replaced by a record of their arguments."""
+import weakref
+
 import pytest
 import torch
 
@@ -195,3 +197,16 @@ def test_groups_are_looked_at_apart(record, clip):
     expect(record.steps[-1], params[1:], opt)
     if clip:
         assert NormList.calls[-1] == ([p.grad.data_ptr() for p in params], [4, 5, 6])
+
+
+@both
+def test_a_replaced_momentum_is_released_at_once(record, clip):
+    """As where the state is moved to the host to make room on the device until the next step."""
+    params, opt = make([(7,), (7,)], clip)
+    opt.step()
+    refs = [weakref.ref(opt.state[p]["exp_avg"]) for p in params]
+    opt.state[params[0]]["exp_avg"] = opt.state[params[0]]["exp_avg"].double().float()
+    del opt.state[params[1]]["exp_avg"]
+    assert [r() for r in refs] == [None, None]
+    opt.step()
+    expect(record.steps[-1], params, opt)
