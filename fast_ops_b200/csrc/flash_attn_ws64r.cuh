@@ -497,7 +497,8 @@ attn_fwd_ws64r_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
       alpha_slot[u * 128] = alpha;
       mbar_arrive(bar_corr + 2 * s + u);
       if ((warp & 3) == 0) trace_event(prm, s, t, 2);
-      // P (two 16-bit values per column) over the first 32 columns of this step's buffer
+      // P (two 16-bit values per column) over the first 32 columns of this step's buffer, rounded to the type of V, as
+      // the tensor core takes both operands of a 16-bit matmul in one type; the row's sum is of P unrounded
       tmem_st16(tS, pr[0]);
       tmem_st16(tS + 16, pr[1]);
       if (more) {
